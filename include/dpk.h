@@ -361,6 +361,47 @@ int dpk_layer_norm_gs(const void* x, const void* b, int in_dtype, void* gs_w, vo
                       dpk_stream_t stream);
 
 /* ------------------------------------------------------------------------- *
+ * The gated linear recurrence of the DPGatedRNN layer. The reference has no such layer; it
+ * stands beside its recurrent layers (opacus/layers/dp_rnn.py), whose gates read the state
+ * and so cannot be scanned.
+ * ------------------------------------------------------------------------- */
+
+/* gates: [n,T,3D] of `dtype`, the values x, the decay gates r and the input gates i of each
+ * position side by side; element (b,t,c) at b * gates_stride_n + t * gates_stride_t + c (strides
+ * in elements, so that a slice of a longer tensor needs no copy). decay: [D] of `decay_dtype`.
+ *   a = exp(-softplus(decay) * sigmoid(r)),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t
+ *   out[b,t,:] = h_t (rounded once to `dtype`),  last[b,:] = the state after the last position
+ * state: float[n,D], the state before the first position (NULL: zeros). lengths: int64[n] or NULL;
+ * positions t >= lengths[b] (clamped to [0,T]) are padding: never read, out is 0 there and the
+ * state is carried over them. reverse != 0 runs t from T-1 down to 0. State and gate arithmetic are
+ * fp32. kept (NULL unless a backward pass follows): float[n, ceil(T / DPK_SCAN_CHUNK), D], the
+ * state before every DPK_SCAN_CHUNK-th position in the order of the scan.
+ * n == 0 or D == 0 launches nothing; T == 0 writes last only. Tensors need their element size's
+ * alignment; wider alignment (and D, strides in multiples of 4 or 2) takes wider loads.
+ * ws: dpk_gated_scan_workspace_bytes bytes (one query for both directions), 16-byte aligned. */
+#define DPK_SCAN_CHUNK 64
+size_t dpk_gated_scan_workspace_bytes(int64_t n, int64_t T, int64_t D);
+int dpk_gated_scan(const void* gates, int dtype, const void* decay, int decay_dtype, const float* state,
+                   const int64_t* lengths, void* out, float* last, float* kept, int64_t n, int64_t T, int64_t D,
+                   int64_t gates_stride_n, int64_t gates_stride_t, int reverse, void* ws, size_t ws_bytes,
+                   dpk_stream_t stream);
+
+/* Gradients of the above from grad_out: [n,T,D] of `dtype` (dense) and grad_last: float[n,D] or
+ * NULL. grad_gates: [n,T,3D] of `dtype` (dense, zero at padding). grad_decay (nullable): float[n,D],
+ * the PER-SAMPLE gradient of decay, which the same pass yields. grad_state (nullable): float[n,D].
+ * gates, decay, lengths, reverse as given to dpk_gated_scan, kept as it left it. */
+int dpk_gated_scan_backward(const void* gates, int dtype, const void* decay, int decay_dtype, const float* kept,
+                            const int64_t* lengths, const void* grad_out, const float* grad_last, void* grad_gates,
+                            float* grad_decay, float* grad_state, int64_t n, int64_t T, int64_t D,
+                            int64_t gates_stride_n, int64_t gates_stride_t, int reverse, void* ws, size_t ws_bytes,
+                            dpk_stream_t stream);
+
+/* One position: gates [n,3D], rows gates_stride_n apart; state float[n,D] is advanced in place and
+ * out[n,D] receives it rounded to `dtype`. */
+int dpk_gated_scan_step(const void* gates, int dtype, const void* decay, int decay_dtype, float* state, void* out,
+                        int64_t n, int64_t D, int64_t gates_stride_n, dpk_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
  * DPOptimizer.clip_and_accumulate, add_noise, scale_grad
  * replaces opacus/optimizers/optimizer.py:432-504
  * ------------------------------------------------------------------------- */

@@ -887,6 +887,161 @@ def layer_norm_grad_sample(
     return (_with_sumsq(gw, ssw) if want_weight else None), (_with_sumsq(gb, ssb) if want_bias else None)
 
 
+# ---- gated linear recurrence ----------------------------------------------------------
+@contextmanager
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device around a launch: a kernel goes to the current device, and
+    the tensors may live on another one."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        yield
+    else:
+        with torch.cuda.device(dev):
+            yield
+
+
+def _gates_layout(gates: torch.Tensor, D: int) -> Tuple[torch.Tensor, int, int]:
+    """``gates`` with unit stride along its features, and its sample and position strides."""
+    if gates.numel() and (gates.stride(-1) != 1 or min(gates.stride()) < 0):
+        gates = gates.contiguous()
+    n, T = gates.shape[0], gates.shape[1]
+    return gates, (gates.stride(0) if n > 1 else T * 3 * D), (gates.stride(1) if T > 1 else 3 * D)
+
+
+def _scan_args(gates, decay, lengths, dims: int):
+    dev = _need_gpu(gates, decay, lengths)
+    if gates.dim() != dims:
+        raise ValueError(f"gates must have {dims} dimensions, got {tuple(gates.shape)}")
+    if decay.dim() != 1 or gates.shape[-1] != 3 * decay.shape[0]:
+        raise ValueError(f"gates {tuple(gates.shape)} must end in 3 * D features for decay {tuple(decay.shape)}")
+    _code(gates), _code(decay)
+    if lengths is not None:
+        if lengths.dtype != torch.int64 or tuple(lengths.shape) != (gates.shape[0],):
+            raise ValueError(f"lengths must be int64 of shape ({gates.shape[0]},), got {lengths.dtype} {tuple(lengths.shape)}")
+        lengths = _dense(lengths)
+    return dev, _dense(decay), lengths
+
+
+def _scan_state(name: str, t: Optional[torch.Tensor], shape, dev) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if _need_gpu(t) != dev:
+        raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
+    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be float32 of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return _dense(t)
+
+
+def gated_scan(
+    gates: torch.Tensor,
+    decay: torch.Tensor,
+    state: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None,
+    reverse: bool = False,
+    keep_states: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """``h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t`` with
+    ``a = exp(-softplus(decay) sigmoid(r))`` along the middle dimension of
+    ``gates = [x | r | i]`` ``[n, T, 3 D]``.
+
+    Returns ``(out, last, kept)``: the states ``[n, T, D]`` in the gates' dtype, the last one
+    ``[n, D]`` in float32, and with ``keep_states`` what :func:`gated_scan_backward` needs. ``state``
+    (float32 ``[n, D]``) comes before the first position. ``lengths`` (int64 ``[n]``) marks
+    positions from ``lengths[b]`` on as padding, which is never read: the state passes over it and
+    the output is zero there. ``reverse`` scans from the last position to the first. ``gates``
+    may be a slice of a larger tensor (any strides but along the features)."""
+    dev, decay, lengths = _scan_args(gates, decay, lengths, 3)
+    n, T, D = gates.shape[0], gates.shape[1], decay.shape[0]
+    state = _scan_state("state", state, (n, D), dev)
+    out = torch.empty((n, T, D), dtype=gates.dtype, device=dev)
+    last = torch.empty((n, D), dtype=torch.float32, device=dev)
+    kept = torch.empty((n, -(-T // _lib.DPK_SCAN_CHUNK), D), dtype=torch.float32, device=dev) if keep_states else None
+    if n == 0 or D == 0:
+        return out, last, kept
+    gates, sn, st = _gates_layout(gates, D)
+    L = lib()
+    ws, wsb = _ws(L.dpk_gated_scan_workspace_bytes(n, T, D), dev)
+    with _on(dev), _timed("gated_scan", dev):
+        check(
+            "dpk_gated_scan",
+            L.dpk_gated_scan(
+                _ptr(gates), _code(gates), _ptr(decay), _code(decay), _ptr(state), _ptr(lengths), _ptr(out), _ptr(last),
+                _ptr(kept), n, T, D, sn, st, int(bool(reverse)), _ptr(ws), wsb, _stream(dev),
+            ),
+        )
+    return out, last, kept
+
+
+def gated_scan_backward(
+    gates: torch.Tensor,
+    decay: torch.Tensor,
+    kept: torch.Tensor,
+    grad_out: torch.Tensor,
+    grad_last: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None,
+    reverse: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of :func:`gated_scan`: ``(grad_gates [n, T, 3 D], grad_decay [n, D],
+    grad_state [n, D])``, the last two in float32. ``grad_decay`` is the per-sample gradient of
+    ``decay``: the pass that forms the gate gradients has it on the way. ``kept`` is what
+    ``gated_scan(..., keep_states=True)`` returned for the same gates, decay, lengths and direction;
+    ``grad_last`` (float32) is the gradient of the last state."""
+    dev, decay, lengths = _scan_args(gates, decay, lengths, 3)
+    n, T, D = gates.shape[0], gates.shape[1], decay.shape[0]
+    _need_gpu(gates, kept, grad_out)
+    if tuple(grad_out.shape) != (n, T, D):
+        raise ValueError(f"grad_out must be {(n, T, D)}, got {tuple(grad_out.shape)}")
+    if grad_out.dtype != gates.dtype:
+        grad_out = grad_out.to(gates.dtype)
+    kept = _scan_state("kept", kept, (n, -(-T // _lib.DPK_SCAN_CHUNK), D), dev)
+    grad_last = _scan_state("grad_last", grad_last, (n, D), dev)
+    grad_gates = torch.empty((n, T, 3 * D), dtype=gates.dtype, device=dev)
+    grad_decay = torch.empty((n, D), dtype=torch.float32, device=dev)
+    grad_state = torch.empty((n, D), dtype=torch.float32, device=dev)
+    if n == 0 or D == 0:
+        return grad_gates, grad_decay, grad_state
+    gates, sn, st = _gates_layout(gates, D)
+    grad_out = _dense(grad_out)
+    L = lib()
+    ws, wsb = _ws(L.dpk_gated_scan_workspace_bytes(n, T, D), dev)
+    with _on(dev), _timed("gated_scan_backward", dev):
+        check(
+            "dpk_gated_scan_backward",
+            L.dpk_gated_scan_backward(
+                _ptr(gates), _code(gates), _ptr(decay), _code(decay), _ptr(kept), _ptr(lengths), _ptr(grad_out),
+                _ptr(grad_last), _ptr(grad_gates), _ptr(grad_decay), _ptr(grad_state), n, T, D, sn, st,
+                int(bool(reverse)), _ptr(ws), wsb, _stream(dev),
+            ),
+        )
+    return grad_gates, grad_decay, grad_state
+
+
+def gated_scan_step(gates: torch.Tensor, decay: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+    """One position of :func:`gated_scan`: ``gates`` ``[n, 3 D]``; ``state`` (dense float32
+    ``[n, D]``) is advanced in place and returned rounded to the gates' dtype."""
+    dev, decay, _ = _scan_args(gates, decay, None, 2)
+    n, D = gates.shape[0], decay.shape[0]
+    if not state.is_contiguous():
+        raise ValueError("state is advanced in place and must be dense")
+    if state.requires_grad and torch.is_grad_enabled():
+        raise ValueError("gated_scan_step advances its state in place and is not differentiable: use gated_scan")
+    _scan_state("state", state, (n, D), dev)
+    out = torch.empty((n, D), dtype=gates.dtype, device=dev)
+    if n == 0 or D == 0:
+        return out
+    if gates.stride(1) != 1 or gates.stride(0) < 0:
+        gates = gates.contiguous()
+    with _on(dev), _timed("gated_scan_step", dev):
+        check(
+            "dpk_gated_scan_step",
+            lib().dpk_gated_scan_step(
+                _ptr(gates), _code(gates), _ptr(decay), _code(decay), _ptr(state), _ptr(out), n, D,
+                gates.stride(0) if n > 1 else 3 * D, _stream(dev),
+            ),
+        )
+    torch.autograd.graph.increment_version(state)
+    return out
+
+
 # ---- optimizer: norms, clip factor, clip-weighted sum, noise ---------------------------
 def _flat2d(gs: torch.Tensor) -> torch.Tensor:
     g = _dense(gs)

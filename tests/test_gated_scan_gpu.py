@@ -1,0 +1,297 @@
+"""The gated scan kernels against the definition in float64 (tests/_scan_reference.py)."""
+
+import pytest
+import torch
+
+from _scan_reference import assert_within, scan_reference
+
+pytestmark = pytest.mark.gpu
+
+
+def make(n, T, D, dtype, seed=0, ragged=False, with_state=False, wide=False):
+    g = torch.Generator().manual_seed(seed * 7919 + n * 131 + T * 17 + D)
+    gates = torch.randn(n, T, 3 * D, generator=g)
+    if wide:  # gates that close and open all the way, decays beyond the series' range
+        gates = gates * 2.5
+        decay = torch.randn(D, generator=g) * 3.0
+    else:
+        decay = torch.log(torch.expm1(-2.0 * torch.log(0.9 + 0.099 * torch.rand(D, generator=g))))
+    gates = gates.clamp(-8, 8).to(dtype).cuda()
+    state = torch.randn(n, D, generator=g).cuda() if with_state else None
+    lengths = None
+    if ragged:
+        lengths = torch.randint(0, T + 1, (n,), generator=g)
+        lengths[0] = 0
+        if n > 1:
+            lengths[1] = min(1, T)
+        if n > 2:
+            lengths[2] = T
+        lengths = lengths.cuda()
+    dy = (torch.randn(n, T, D, generator=g) * 0.05).to(dtype).cuda()
+    dl = torch.randn(n, D, generator=g).cuda() if with_state else None
+    return gates, decay.cuda(), state, lengths, dy, dl
+
+
+def check(gates, decay, state, lengths, dy, dl, reverse=False):
+    from opacus_amd import kernels
+
+    out, last, kept = kernels.gated_scan(gates, decay, state, lengths, reverse, keep_states=True)
+    out2, last2, none = kernels.gated_scan(gates, decay, state, lengths, reverse)
+    assert none is None and torch.equal(out, out2) and torch.equal(last, last2)
+    dg, dd, ds = kernels.gated_scan_backward(gates, decay, kept, dy, dl, lengths, reverse)
+    again = kernels.gated_scan_backward(gates, decay, kept, dy, dl, lengths, reverse)
+    assert all(torch.equal(p, q) for p, q in zip((dg, dd, ds), again))  # fixed order: the same bits
+    val, tol = scan_reference(gates, decay, state, lengths, reverse, dy, dl)
+    for name, got in (("out", out), ("last", last), ("grad_gates", dg), ("grad_decay", dd), ("grad_state", ds)):
+        assert_within(got, val[name], tol[name], name)
+
+
+SHAPES = [
+    (1, 1, 1), (1, 1, 64), (3, 2, 5), (2, 7, 4), (2, 8, 66), (2, 9, 64), (1, 63, 3), (1, 64, 16), (2, 65, 65), (1, 127, 34),
+    (2, 128, 64), (1, 129, 130), (5, 200, 20), (1, 1025, 8), (2, 700, 72), (1, 2500, 6),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,T,D", SHAPES)
+def test_shapes(n, T, D, dtype):
+    check(*make(n, T, D, dtype))
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,T,D", [(4, 5, 6), (6, 150, 68), (3, 1500, 10), (5, 64, 33)])
+def test_padded_batches_states_and_directions(n, T, D, dtype, reverse):
+    check(*make(n, T, D, dtype, ragged=True, with_state=True), reverse=reverse)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gates_and_decays_over_their_whole_range(dtype):
+    check(*make(3, 300, 48, dtype, with_state=True, wide=True))
+
+
+def test_many_rows_leave_the_time_axis_whole():
+    check(*make(40, 140, 1024, torch.bfloat16))
+
+
+def test_slices_and_unaligned_views_are_read_in_place():
+    gates, decay, state, lengths, dy, dl = make(4, 90, 24, torch.bfloat16, ragged=True, with_state=True)
+    big = torch.full((9, 95, 80), float("nan"), dtype=torch.bfloat16, device="cuda")
+    view = big[1::2, 3:93, 5:77]  # odd offset, strides that are no multiple of the vector width
+    view.copy_(gates)
+    check(view, decay, state, lengths, dy, dl)
+    by_time = gates.transpose(0, 1).contiguous().transpose(0, 1)  # [T, n, 3D] storage
+    check(by_time, decay, state, lengths, dy, dl)
+    check(gates[..., ::1].flip(2).flip(2), decay, state, lengths, dy.transpose(0, 1).contiguous().transpose(0, 1), dl)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_padding_is_never_read_and_comes_out_as_zero(reverse):
+    from opacus_amd import kernels
+
+    gates, decay, state, lengths, dy, dl = make(5, 130, 20, torch.float32, ragged=True, with_state=True)
+    dead = torch.arange(130, device="cuda")[None, :] >= lengths[:, None]
+    want = kernels.gated_scan(gates, decay, state, lengths, reverse, keep_states=True)
+    want_b = kernels.gated_scan_backward(gates, decay, want[2], dy, dl, lengths, reverse)
+    for bad in (float("nan"), float("inf"), torch.finfo(torch.float32).min):
+        gb, yb = gates.clone(), dy.clone()
+        gb[dead], yb[dead] = bad, bad
+        got = kernels.gated_scan(gb, decay, state, lengths, reverse, keep_states=True)
+        got_b = kernels.gated_scan_backward(gb, decay, got[2], yb, dl, lengths, reverse)
+        for p, q in zip(got + got_b, want + want_b):
+            assert torch.equal(p, q)
+        assert (got[0][dead] == 0).all() and (got_b[0][dead] == 0).all()
+    # a sequence of length zero: the state as it came, its gradient as it came
+    assert torch.equal(want[1][0], state[0]) and torch.equal(want_b[2][0], dl[0]) and (want_b[1][0] == 0).all()
+
+
+def test_lengths_outside_the_range_are_clamped():
+    from opacus_amd import kernels
+
+    gates, decay, *_ = make(3, 20, 8, torch.float32)
+    bad = torch.tensor([-5, 21, 2**40], device="cuda")
+    good = torch.tensor([0, 20, 20], device="cuda")
+    for p, q in zip(kernels.gated_scan(gates, decay, None, bad)[:2], kernels.gated_scan(gates, decay, None, good)[:2]):
+        assert torch.equal(p, q)
+
+
+def test_closed_gates_have_finite_gradients():
+    from opacus_amd import kernels
+
+    gates, decay, *_ = make(2, 40, 8, torch.float32)
+    gates[..., 8:16] = torch.tensor([-200.0, -90.0, float("-inf"), -30.0, 200.0, float("inf"), 90.0, 0.0], device="cuda")
+    decay = torch.tensor([0.5, -120.0, 3.0, -60.0, 40.0, -20.0, 100.0, -200.0], device="cuda")
+    out, last, kept = kernels.gated_scan(gates, decay, keep_states=True)
+    dg, dd, ds = kernels.gated_scan_backward(gates, decay, kept, torch.ones_like(out))
+    for t in (out, last, dg, dd, ds):
+        assert torch.isfinite(t).all()
+
+
+def test_not_a_number_goes_forward_only():
+    from opacus_amd import kernels
+
+    gates, decay, *_ = make(1, 200, 4, torch.float32)
+    clean = kernels.gated_scan(gates, decay)[0]
+    gates[0, 100, 1] = float("nan")
+    out = kernels.gated_scan(gates, decay)[0]
+    assert torch.equal(out[:, :100], clean[:, :100]) and torch.equal(out[..., [0, 2, 3]], clean[..., [0, 2, 3]])
+    assert out[0, 100:, 1].isnan().all()
+
+
+def test_empty_sizes():
+    from opacus_amd import kernels
+
+    for dtype in (torch.float32, torch.bfloat16):
+        for n, T, D in ((0, 5, 4), (3, 0, 4), (3, 5, 0), (0, 0, 4)):
+            gates, decay = torch.zeros(n, T, 3 * D, dtype=dtype, device="cuda"), torch.zeros(D, device="cuda")
+            state = torch.randn(n, D, device="cuda")
+            out, last, kept = kernels.gated_scan(gates, decay, state, keep_states=True)
+            dg, dd, ds = kernels.gated_scan_backward(gates, decay, kept, out, state)
+            assert out.shape == (n, T, D) and dg.shape == gates.shape and dd.shape == (n, D)
+            if T == 0:
+                assert torch.equal(last, state) and torch.equal(ds, state) and (dd == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,D", [(1, 1), (1, 2048), (7, 130), (250, 33), (64, 1000)])
+def test_step_is_one_position_of_the_scan(n, D, dtype):
+    from opacus_amd import kernels
+
+    gates, decay, state, _, _, _ = make(n, 1, D, dtype, with_state=True)
+    val, tol = scan_reference(gates, decay, state)
+    run = state.clone()
+    version = run._version
+    out = kernels.gated_scan_step(gates[:, 0], decay, run)
+    assert run._version > version
+    assert_within(out, val["out"][:, 0], tol["out"][:, 0], "out")
+    assert_within(run, val["last"], tol["last"], "state")
+
+
+def test_steps_after_a_prefix_continue_the_scan():
+    from opacus_amd import kernels
+
+    gates, decay, state, _, _, _ = make(3, 70, 40, torch.float32, with_state=True)
+    whole = kernels.gated_scan(gates, decay, state)[0]
+    _, run, _ = kernels.gated_scan(gates[:, :50], decay, state)
+    val, tol = scan_reference(gates, decay, state)
+    for t in range(50, 70):
+        out = kernels.gated_scan_step(gates[:, t], decay, run)  # rows of a longer tensor, read with its stride
+        assert_within(out, val["out"][:, t], tol["out"][:, t], f"step {t}")
+    assert_within(whole, val["out"], tol["out"], "whole")
+
+
+def test_bfloat16_decay_and_gradients_by_differences():
+    """The float32 kernels' gradient against central differences of the float64 definition."""
+    from opacus_amd import kernels
+
+    gates, decay, state, lengths, dy, dl = make(2, 12, 3, torch.float32, ragged=True, with_state=True)
+    decay = decay.to(torch.bfloat16)
+    check(gates, decay, state, lengths, dy, dl)
+    _, _, kept = kernels.gated_scan(gates, decay, state, lengths, keep_states=True)
+    dg, dd, ds = kernels.gated_scan_backward(gates, decay, kept, dy, dl, lengths)
+
+    import _scan_reference as R
+
+    def loss(g, lam, s):
+        keep, R.half_step = R.half_step, lambda dtype: R.H
+        try:
+            val, _ = scan_reference(g, lam, s, lengths)
+        finally:
+            R.half_step = keep
+        return (val["out"] * dy.double().cpu()).sum((1, 2)) + (val["last"] * dl.double().cpu()).sum(1)
+
+    base = [gates.double().cpu(), decay.double().cpu(), state.double().cpu()]
+    step = 1e-5  # central differences: truncation about step^2 = 1e-10, rounding 1e-16 / step = 1e-11 of values near 1
+    for which, grad in enumerate((dg, dd, ds)):
+        grad = grad.double().cpu()
+        shape = base[which].shape if which != 1 else (2, 3)
+        for idx in range(grad.numel()):
+            lo, hi = [t.clone() for t in base], [t.clone() for t in base]
+            at = idx if which != 1 else idx % 3
+            lo[which].view(-1)[at] -= step
+            hi[which].view(-1)[at] += step
+            d = (loss(*hi) - loss(*lo)) / (2 * step)
+            want = d[idx // (grad.numel() // shape[0])] if which != 1 else d[idx // 3]
+            assert abs(grad.reshape(-1)[idx] - want) <= 2e-5 * (1 + abs(want)), (which, idx)
+
+
+def test_refusals_on_the_gpu():
+    from opacus_amd import kernels
+
+    gates, decay, state, lengths, dy, _ = make(2, 6, 4, torch.float32, ragged=True, with_state=True)
+    _, _, kept = kernels.gated_scan(gates, decay, keep_states=True)
+    with pytest.raises(ValueError, match="dimensions"):
+        kernels.gated_scan(gates[0], decay)
+    with pytest.raises(ValueError, match="3 \\* D"):
+        kernels.gated_scan(gates, decay[:3])
+    with pytest.raises(ValueError, match="state"):
+        kernels.gated_scan(gates, decay, state.bfloat16())
+    with pytest.raises(ValueError, match="state"):
+        kernels.gated_scan(gates, decay, state[:1])
+    with pytest.raises(ValueError, match="lengths"):
+        kernels.gated_scan(gates, decay, None, lengths.int())
+    with pytest.raises(ValueError, match="lengths"):
+        kernels.gated_scan(gates, decay, None, lengths[:1])
+    with pytest.raises(TypeError):
+        kernels.gated_scan(gates.half(), decay)
+    with pytest.raises(TypeError):
+        kernels.gated_scan(gates, decay.double())
+    with pytest.raises(RuntimeError, match="GPU only"):
+        kernels.gated_scan(gates, decay.cpu())
+    with pytest.raises(ValueError, match="kept"):
+        kernels.gated_scan_backward(gates, decay, kept[:, :0], dy)
+    with pytest.raises(ValueError, match="grad_out"):
+        kernels.gated_scan_backward(gates, decay, kept, dy[:, :3])
+    with pytest.raises(ValueError, match="grad_last"):
+        kernels.gated_scan_backward(gates, decay, kept, dy, state[:, :2])
+    with pytest.raises(ValueError, match="dense"):
+        kernels.gated_scan_step(gates[:, 0], decay, state.t().contiguous().t())
+    with pytest.raises(ValueError, match="not differentiable"):
+        kernels.gated_scan_step(gates[:, 0], decay, state.clone().requires_grad_(True))
+
+
+def test_captured_calls_replay_on_new_inputs():
+    from opacus_amd import kernels
+
+    # one shape that cuts T into segments (workspace inside the graph's pool), two graphs alive at once
+    sets = [make(1, 1500, 64, torch.bfloat16, seed=s, with_state=True) for s in range(4)]
+    gates, decay, state, _, dy, dl = (t.clone() if t is not None else None for t in sets[0])
+
+    def call():
+        out, last, kept = kernels.gated_scan(gates, decay, state, keep_states=True)
+        return (out, last) + kernels.gated_scan_backward(gates, decay, kept, dy, dl)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = call()
+        graphs.append((g, res))
+    for k in (1, 2, 3, 1):
+        for dst, src in zip((gates, decay, state, dy, dl), (sets[k][0], sets[k][1], sets[k][2], sets[k][4], sets[k][5])):
+            dst.copy_(src)
+        want = [t.clone() for t in call()]
+        for g, res in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, res in graphs:
+            for p, q in zip(res, want):
+                assert torch.equal(p, q)
+
+
+def test_another_stream():
+    from opacus_amd import kernels
+
+    gates, decay, state, lengths, dy, dl = make(2, 300, 64, torch.bfloat16, ragged=True, with_state=True)
+    want = kernels.gated_scan(gates, decay, state, lengths)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = kernels.gated_scan(gates, decay, state, lengths)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(p, q) for p, q in zip(got[:2], want[:2]))
