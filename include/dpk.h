@@ -402,6 +402,37 @@ int dpk_gated_scan_step(const void* gates, int dtype, const void* decay, int dec
                         int64_t n, int64_t D, int64_t gates_stride_n, dpk_stream_t stream);
 
 /* ------------------------------------------------------------------------- *
+ * Group normalisation with an activation on channels-last tensors. The forward and the input
+ * gradient are torch's in the reference; the per-sample parameter gradients are
+ * opacus/grad_sample/group_norm.py:26-47.
+ * ------------------------------------------------------------------------- */
+
+enum dpk_act { DPK_ACT_NONE = 0, DPK_ACT_RELU = 1, DPK_ACT_SILU = 2, DPK_ACT_GELU = 3 /* erf form */ };
+
+/* x, y: [n,S,C] of `dtype`, channels last (the memory of a channels_last image with S = H * W, or of
+ * a batch of token rows). y = act(weight * (x - mean) * rstd + bias), the statistics (biased variance,
+ * eps >= 0 added) over groups of C / groups neighbouring channels and
+ *   per_position == 0: all S positions of the sample (nn.GroupNorm);
+ *   per_position == 1: one position (every head of a token on its own).
+ * weight, bias: [C] of `param_dtype`, or NULL for 1 and 0. stats: float[n,groups,2] (mean, rstd),
+ * 8-byte aligned, written for the backward pass; not used (NULL) with per_position.
+ * Statistics and sums are fp32. n == 0 or S == 0 launches nothing. Tensors need their element
+ * size's alignment; wider alignment and channel counts take wider loads.
+ * ws: dpk_group_norm_act_workspace_bytes bytes (one query for both directions), 16-byte aligned. */
+size_t dpk_group_norm_act_workspace_bytes(int64_t n, int64_t S, int64_t C, int64_t groups, int per_position);
+int dpk_group_norm_act(const void* x, int dtype, const void* weight, const void* bias, int param_dtype, void* y,
+                       float* stats, int64_t n, int64_t S, int64_t C, int64_t groups, float eps, int act,
+                       int per_position, void* ws, size_t ws_bytes, dpk_stream_t stream);
+
+/* Gradients of the above: grad_x [n,S,C] of `dtype`; grad_weight and grad_bias (nullable): float[n,C],
+ * the PER-SAMPLE gradients, formed by the pass over x and grad_out that the input gradient needs
+ * anyway. stats as dpk_group_norm_act left it (NULL with per_position). */
+int dpk_group_norm_act_backward(const void* x, const void* grad_out, int dtype, const void* weight, const void* bias,
+                                int param_dtype, const float* stats, void* grad_x, float* grad_weight,
+                                float* grad_bias, int64_t n, int64_t S, int64_t C, int64_t groups, float eps, int act,
+                                int per_position, void* ws, size_t ws_bytes, dpk_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
  * DPOptimizer.clip_and_accumulate, add_noise, scale_grad
  * replaces opacus/optimizers/optimizer.py:432-504
  * ------------------------------------------------------------------------- */

@@ -24,6 +24,7 @@ DPK_ROUTE_AUTO, DPK_ROUTE_GRAM, DPK_ROUTE_DIRECT = 0, 1, 2
 DPK_STATIC_SCRATCH_BYTES = 8 << 20
 DPK_GHOST_MULTI_MAX = 256
 DPK_SCAN_CHUNK = 64
+DPK_ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 class GhostLayer(ctypes.Structure):
@@ -121,6 +122,13 @@ SIGNATURES = {
         c_int, [_P, c_int, _P, c_int] + [_P] * 7 + [_I] * 5 + [c_int, _P, c_size_t, _P]
     ),
     "dpk_gated_scan_step": (c_int, [_P, c_int, _P, c_int, _P, _P, _I, _I, _I, _P]),
+    "dpk_group_norm_act_workspace_bytes": (c_size_t, [_I, _I, _I, _I, c_int]),
+    "dpk_group_norm_act": (
+        c_int, [_P, c_int, _P, _P, c_int, _P, _P, _I, _I, _I, _I, c_float, c_int, c_int, _P, c_size_t, _P]
+    ),
+    "dpk_group_norm_act_backward": (
+        c_int, [_P, _P, c_int, _P, _P, c_int, _P, _P, _P, _P, _I, _I, _I, _I, c_float, c_int, c_int, _P, c_size_t, _P]
+    ),
     "dpk_sumsq_rows_workspace_bytes": (c_size_t, [_I, _I]),
     "dpk_sumsq_rows": (c_int, [_P, c_int, _I, _I, _P, _P, c_size_t, _P]),
     "dpk_clip_factor": (c_int, [_P, _I, _I, c_int, c_float, _P, _P, _P]),

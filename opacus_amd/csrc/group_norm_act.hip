@@ -1,0 +1,656 @@
+// Group normalisation with an affine map and an activation on channels-last tensors, forward and
+// backward, the backward pass with PER-SAMPLE weight and bias gradients.
+//
+//   x[n,S,C], G groups of Cg = C / G neighbouring channels;  xh = (x - mu) rstd;  z = w xh + b;  y = act(z)
+//   dz = dy act'(z);  gw[n,c] = sum_s dz xh;  gb[n,c] = sum_s dz
+//   dx = rstd (w dz - S1 - xh S2),  S1 = mean of w dz, S2 = mean of w dz xh over the statistics' elements
+//
+// Statistics per sample (nn.GroupNorm: over all S positions and the group's channels): S1 and S2
+// are sums over the group's channels of w gb and w gw, so the per-sample parameter gradients that a
+// DP step needs ARE the sums the input gradient waits for, and one reading of x and dy forms both.
+// Statistics per position (each position's groups on their own, a norm per attention or recurrence
+// head): the sums stay within a few lanes, and gw, gb are kept in registers along the rows.
+//
+// Means and variances are two-step (the mean first, then squares around it) within what a thread
+// holds, and put together from (count, mean, M2) triples, so that a large mean costs no digits.
+// All arithmetic is fp32; every reduction runs in a fixed order.
+#include <type_traits>
+
+#include "vec_io.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 8;           // rows a thread has in flight in the streaming kernels
+constexpr int64_t kWantBlocks = 2048;
+
+constexpr int kRelu = DPK_ACT_RELU, kSilu = DPK_ACT_SILU, kGelu = DPK_ACT_GELU;
+
+// z -> act(z) for N values; one uniform branch for all of them.
+template <int N>
+__device__ __forceinline__ void activate(float (&z)[N], int act) {
+  if (act == kSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] *= sigmoid_f(z[i]);
+  } else if (act == kGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] *= 0.5f * (1.0f + erff(z[i] * 0.70710678118654752f));
+  } else if (act == kRelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : (z[i] != z[i] ? z[i] : 0.f);
+  }
+}
+// z -> act'(z)
+template <int N>
+__device__ __forceinline__ void slope(float (&z)[N], int act) {
+  if (act == kSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float s = sigmoid_f(z[i]);
+      z[i] = s * fmaf(z[i], 1.0f - s, 1.0f);
+    }
+  } else if (act == kGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float phi = 0.5f * (1.0f + erff(z[i] * 0.70710678118654752f));
+      z[i] = fmaf(z[i] * 0.39894228040143268f, __builtin_amdgcn_exp2f(z[i] * z[i] * (-0.5f * kLog2e)), phi);
+    }
+  } else if (act == kRelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? 1.0f : (z[i] != z[i] ? z[i] : 0.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = 1.0f;
+  }
+}
+
+struct NormArgs {
+  const void* x;
+  const void* dy;
+  const void* w;        // null: 1
+  const void* b;        // null: 0
+  void* y;              // or dx
+  float2* stats;        // [n,G] (mean, rstd); per position [n*S,G] in the workspace
+  float2* part;         // [n,J,C] (mean, M2) or (sum dz, sum dz xh)
+  float2* sums;         // [n,G] (S1, S2)
+  float* gw;            // [n,C] or null
+  float* gb;
+  int64_t n, S;
+  int C, G, Cg;
+  int cl;               // vectors of a row that a block covers
+  int cblocks;          // blocks along a row
+  int J;                // row chunks of a sample
+  int64_t chunk;        // rows of one
+  int param_bf16, act;
+  float eps;
+};
+
+__device__ __forceinline__ float param_at(const void* p, int is_bf16, int c, float none) {
+  if (!p) return none;
+  return is_bf16 ? bf16_to_f32(static_cast<const bf16_t*>(p)[c]) : static_cast<const float*>(p)[c];
+}
+
+// What a thread of the streaming kernels works on: vector column c of rows r0 + rg, r0 + rg + step, ...
+struct Span {
+  int64_t b, r0, r1;
+  int c, rg, step, j;
+  bool on;
+};
+template <int V>
+__device__ __forceinline__ Span span_of(const NormArgs& p) {
+  Span s;
+  int64_t bid = blockIdx.x;
+  const int cb = static_cast<int>(bid % p.cblocks);
+  bid /= p.cblocks;
+  s.j = static_cast<int>(bid % p.J);
+  s.b = bid / p.J;
+  const int lane = threadIdx.x % p.cl;
+  s.rg = threadIdx.x / p.cl;
+  s.step = kThreads / p.cl;
+  s.c = (cb * p.cl + lane) * V;
+  s.on = s.rg < s.step && s.c < p.C;
+  s.r0 = s.j * p.chunk;
+  s.r1 = s.r0 + p.chunk < p.S ? s.r0 + p.chunk : p.S;
+  return s;
+}
+
+// ---- statistics per sample: partial sums, merged sums, application ------------------------
+
+// part[n,j,c] = (mean, M2) of channel c over the rows of chunk j.
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void sample_stat_kernel(NormArgs p) {
+  typedef vec_io<T, V> io;
+  __shared__ float lds[2][kThreads][V];
+  const Span s = span_of<V>(p);
+  const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
+  float mean[V], m2[V], cnt = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.f;
+  if (s.on) {
+    for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * kRows) {
+      typename io::raw raw[kRows];
+      int m = 0;
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int64_t at = r + static_cast<int64_t>(k) * s.step;
+        raw[k] = typename io::raw();
+        if (at < s.r1) {
+          raw[k] = io::load(x + at * p.C);
+          ++m;
+        }
+      }
+      const float fm = static_cast<float>(m), inv = 1.0f / fm, all = cnt + fm, share = fm / all;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) t += k < m ? io::get(raw[k], j) : 0.f;
+        t *= inv;
+        float q = 0.f;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          const float d = k < m ? io::get(raw[k], j) - t : 0.f;
+          q = fmaf(d, d, q);
+        }
+        const float delta = t - mean[j];
+        mean[j] = fmaf(delta, share, mean[j]);
+        m2[j] += q + delta * delta * (cnt * share);
+      }
+      cnt = all;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) lds[0][threadIdx.x][j] = mean[j], lds[1][threadIdx.x][j] = m2[j];
+  __syncthreads();
+  if (s.on && s.rg == 0) {
+    // rows of row group g: ceil((rows - g) / step)
+    const int64_t rows = s.r1 - s.r0;
+    const int lane = threadIdx.x;
+    float2* out = p.part + (s.b * p.J + s.j) * p.C + s.c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float t = 0.f, q = 0.f;
+      for (int g = 0; g < s.step && g < rows; ++g)
+        t += static_cast<float>((rows - g + s.step - 1) / s.step) * lds[0][g * p.cl + lane][j];
+      t /= static_cast<float>(rows);
+      for (int g = 0; g < s.step && g < rows; ++g) {
+        const float d = lds[0][g * p.cl + lane][j] - t;
+        q += fmaf(d * d, static_cast<float>((rows - g + s.step - 1) / s.step), lds[1][g * p.cl + lane][j]);
+      }
+      out[j] = make_float2(t, q);
+    }
+  }
+}
+
+// stats[n,g] from the (mean, M2) of its channels and chunks. One block per (n, g).
+__global__ __launch_bounds__(kThreads) void sample_stat_merge_kernel(NormArgs p) {
+  __shared__ float red[kThreads / DPK_WAVE];
+  __shared__ float share;
+  const int64_t b = blockIdx.x / p.G;
+  const int g = static_cast<int>(blockIdx.x % p.G);
+  const float2* part = p.part + b * p.J * p.C + g * p.Cg;
+  const int items = p.J * p.Cg;
+  const float total = static_cast<float>(p.S) * static_cast<float>(p.Cg);
+  float t = 0.f;
+  for (int i = threadIdx.x; i < items; i += kThreads) {
+    const int j = i / p.Cg;
+    const int64_t rows = p.S - j * p.chunk < p.chunk ? p.S - j * p.chunk : p.chunk;
+    t += static_cast<float>(rows) * part[static_cast<int64_t>(j) * p.C + (i - j * p.Cg)].x;
+  }
+  t = block_sum<kThreads / DPK_WAVE>(t, red);
+  if (threadIdx.x == 0) share = t / total;
+  __syncthreads();
+  const float mean = share;
+  float q = 0.f;
+  for (int i = threadIdx.x; i < items; i += kThreads) {
+    const int j = i / p.Cg;
+    const int64_t rows = p.S - j * p.chunk < p.chunk ? p.S - j * p.chunk : p.chunk;
+    const float2 v = part[static_cast<int64_t>(j) * p.C + (i - j * p.Cg)];
+    const float d = v.x - mean;
+    q += fmaf(d * d, static_cast<float>(rows), v.y);
+  }
+  q = block_sum<kThreads / DPK_WAVE>(q, red);
+  if (threadIdx.x == 0) p.stats[blockIdx.x] = make_float2(mean, 1.0f / sqrtf(q / total + p.eps));
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void sample_apply_kernel(NormArgs p) {
+  typedef vec_io<T, V> io;
+  const Span s = span_of<V>(p);
+  if (!s.on) return;
+  const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
+  T* y = static_cast<T*>(p.y) + (s.b * p.S) * p.C + s.c;
+  float mean[V], f[V], shift[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float2 st = p.stats[s.b * p.G + (s.c + j) / p.Cg];
+    mean[j] = st.x;
+    f[j] = st.y * param_at(p.w, p.param_bf16, s.c + j, 1.f);
+    shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
+  }
+  for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * kRows) {
+    typename io::raw raw[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int64_t at = r + static_cast<int64_t>(k) * s.step;
+      raw[k] = typename io::raw();
+      if (at < s.r1) raw[k] = io::load(x + at * p.C);
+    }
+    float z[kRows * V];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[k * V + j] = fmaf(io::get(raw[k], j) - mean[j], f[j], shift[j]);
+    }
+    activate(z, p.act);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int64_t at = r + static_cast<int64_t>(k) * s.step;
+      if (at < s.r1) io::store(y + at * p.C, z + k * V);
+    }
+  }
+}
+
+// (mean, rstd) of one element's statistics: per sample once per thread, per position from the row.
+template <typename T, int V, bool PER_POSITION>
+__global__ __launch_bounds__(kThreads) void channel_sums_kernel(NormArgs p) {
+  typedef vec_io<T, V> io;
+  constexpr int R = 4;
+  __shared__ float lds[2][kThreads][V];
+  const Span s = span_of<V>(p);
+  const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
+  const T* dy = static_cast<const T*>(p.dy) + (s.b * p.S) * p.C + s.c;
+  float A[V], B[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) A[j] = B[j] = 0.f;
+  if (s.on) {
+    float2 st[V];
+    float w[V], shift[V];
+    int grp[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      grp[j] = (s.c + j) / p.Cg;
+      if (!PER_POSITION) st[j] = p.stats[s.b * p.G + grp[j]];
+      w[j] = param_at(p.w, p.param_bf16, s.c + j, 1.f);
+      shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
+    }
+    for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * R) {
+      typename io::raw rx[R], rd[R];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int64_t at = r + static_cast<int64_t>(k) * s.step;
+        rx[k] = rd[k] = typename io::raw();
+        if (at < s.r1) {
+          rx[k] = io::load(x + at * p.C);
+          rd[k] = io::load(dy + at * p.C);
+        }
+      }
+      float xh[R * V], z[R * V];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int64_t at = r + static_cast<int64_t>(k) * s.step;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (PER_POSITION) st[j] = at < s.r1 ? p.stats[(s.b * p.S + at) * p.G + grp[j]] : make_float2(0.f, 0.f);
+          xh[k * V + j] = (io::get(rx[k], j) - st[j].x) * st[j].y;
+          z[k * V + j] = fmaf(xh[k * V + j], w[j], shift[j]);
+        }
+      }
+      slope(z, p.act);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (r + static_cast<int64_t>(k) * s.step < s.r1) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float dz = io::get(rd[k], j) * z[k * V + j];
+            A[j] += dz;
+            B[j] = fmaf(dz, xh[k * V + j], B[j]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) lds[0][threadIdx.x][j] = A[j], lds[1][threadIdx.x][j] = B[j];
+  __syncthreads();
+  if (s.on && s.rg == 0) {
+    float2* out = p.part + (s.b * p.J + s.j) * p.C + s.c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float t = 0.f, q = 0.f;
+      for (int g = 0; g < s.step; ++g) t += lds[0][g * p.cl + threadIdx.x][j], q += lds[1][g * p.cl + threadIdx.x][j];
+      out[j] = make_float2(t, q);
+    }
+  }
+}
+
+// gw, gb from the chunks' sums, and S1, S2 of the group. One block per (n, g).
+__global__ __launch_bounds__(kThreads) void sample_grad_merge_kernel(NormArgs p) {
+  __shared__ float red[kThreads / DPK_WAVE];
+  const int64_t b = blockIdx.x / p.G;
+  const int g = static_cast<int>(blockIdx.x % p.G);
+  float s1 = 0.f, s2 = 0.f;
+  for (int i = threadIdx.x; i < p.Cg; i += kThreads) {
+    const int c = g * p.Cg + i;
+    const float2* part = p.part + b * p.J * p.C + c;
+    float A = 0.f, B = 0.f;
+    for (int j = 0; j < p.J; ++j) {
+      const float2 v = part[static_cast<int64_t>(j) * p.C];
+      A += v.x;
+      B += v.y;
+    }
+    if (p.gb) p.gb[b * p.C + c] = A;
+    if (p.gw) p.gw[b * p.C + c] = B;
+    const float w = param_at(p.w, p.param_bf16, c, 1.f);
+    s1 = fmaf(w, A, s1);
+    s2 = fmaf(w, B, s2);
+  }
+  s1 = block_sum<kThreads / DPK_WAVE>(s1, red);
+  s2 = block_sum<kThreads / DPK_WAVE>(s2, red);
+  const float inv = 1.0f / (static_cast<float>(p.S) * static_cast<float>(p.Cg));
+  if (threadIdx.x == 0) p.sums[blockIdx.x] = make_float2(s1 * inv, s2 * inv);
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void sample_dx_kernel(NormArgs p) {
+  typedef vec_io<T, V> io;
+  constexpr int R = 4;
+  const Span s = span_of<V>(p);
+  if (!s.on) return;
+  const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
+  const T* dy = static_cast<const T*>(p.dy) + (s.b * p.S) * p.C + s.c;
+  T* dx = static_cast<T*>(p.y) + (s.b * p.S) * p.C + s.c;
+  float2 st[V], sm[V];
+  float w[V], shift[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int64_t g = s.b * p.G + (s.c + j) / p.Cg;
+    st[j] = p.stats[g];
+    sm[j] = p.sums[g];
+    w[j] = param_at(p.w, p.param_bf16, s.c + j, 1.f);
+    shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
+  }
+  for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * R) {
+    typename io::raw rx[R], rd[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int64_t at = r + static_cast<int64_t>(k) * s.step;
+      rx[k] = rd[k] = typename io::raw();
+      if (at < s.r1) {
+        rx[k] = io::load(x + at * p.C);
+        rd[k] = io::load(dy + at * p.C);
+      }
+    }
+    float xh[R * V], z[R * V];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xh[k * V + j] = (io::get(rx[k], j) - st[j].x) * st[j].y;
+        z[k * V + j] = fmaf(xh[k * V + j], w[j], shift[j]);
+      }
+    }
+    slope(z, p.act);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = io::get(rd[k], j) * z[k * V + j] * w[j];
+        o[j] = st[j].y * (d - sm[j].x - xh[k * V + j] * sm[j].y);
+      }
+      const int64_t at = r + static_cast<int64_t>(k) * s.step;
+      if (at < s.r1) io::store(dx + at * p.C, o);
+    }
+  }
+}
+
+// ---- statistics per position, any group size: one wave per (row, group) -----------------------
+
+template <typename T, bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void position_kernel(NormArgs p) {
+  typedef vec_io<T, 1> io;
+  const int64_t wave = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / DPK_WAVE;
+  const int lane = threadIdx.x & (DPK_WAVE - 1);
+  if (wave >= p.n * p.S * p.G) return;
+  const int64_t row = wave / p.G;
+  const int g = static_cast<int>(wave - row * p.G);
+  const int c0 = g * p.Cg;
+  const T* x = static_cast<const T*>(p.x) + row * p.C + c0;
+  T* y = static_cast<T*>(p.y) + row * p.C + c0;
+  const float inv = 1.0f / static_cast<float>(p.Cg);
+  float t = 0.f;
+  for (int i = lane; i < p.Cg; i += DPK_WAVE) t += io::get(x[i], 0);
+  const float mean = wave_sum(t) * inv;
+  t = 0.f;
+  for (int i = lane; i < p.Cg; i += DPK_WAVE) {
+    const float d = io::get(x[i], 0) - mean;
+    t = fmaf(d, d, t);
+  }
+  const float rstd = 1.0f / sqrtf(wave_sum(t) * inv + p.eps);
+  if (!BACKWARD) {
+    for (int i = lane; i < p.Cg; i += DPK_WAVE) {
+      float z[1] = {fmaf((io::get(x[i], 0) - mean) * rstd, param_at(p.w, p.param_bf16, c0 + i, 1.f),
+                         param_at(p.b, p.param_bf16, c0 + i, 0.f))};
+      activate(z, p.act);
+      io::store(y + i, z);
+    }
+    return;
+  }
+  if (lane == 0) p.stats[wave] = make_float2(mean, rstd);
+  const T* dy = static_cast<const T*>(p.dy) + row * p.C + c0;
+  float s1 = 0.f, s2 = 0.f;
+  for (int i = lane; i < p.Cg; i += DPK_WAVE) {
+    const float w = param_at(p.w, p.param_bf16, c0 + i, 1.f), xh = (io::get(x[i], 0) - mean) * rstd;
+    float z[1] = {fmaf(xh, w, param_at(p.b, p.param_bf16, c0 + i, 0.f))};
+    slope(z, p.act);
+    const float d = io::get(dy[i], 0) * z[0] * w;
+    s1 += d;
+    s2 = fmaf(d, xh, s2);
+  }
+  s1 = wave_sum(s1) * inv;
+  s2 = wave_sum(s2) * inv;
+  for (int i = lane; i < p.Cg; i += DPK_WAVE) {
+    const float w = param_at(p.w, p.param_bf16, c0 + i, 1.f), xh = (io::get(x[i], 0) - mean) * rstd;
+    float z[1] = {fmaf(xh, w, param_at(p.b, p.param_bf16, c0 + i, 0.f))};
+    slope(z, p.act);
+    const float o[1] = {rstd * (io::get(dy[i], 0) * z[0] * w - s1 - xh * s2)};
+    io::store(y + i, o);
+  }
+}
+
+// gw, gb[n,c] from the chunks' sums.
+__global__ __launch_bounds__(kThreads) void chunk_merge_kernel(NormArgs p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= p.n * p.C) return;
+  const int64_t b = i / p.C;
+  const float2* part = p.part + b * p.J * p.C + (i - b * p.C);
+  float A = 0.f, B = 0.f;
+  for (int j = 0; j < p.J; ++j) {
+    const float2 v = part[static_cast<int64_t>(j) * p.C];
+    A += v.x;
+    B += v.y;
+  }
+  if (p.gb) p.gb[i] = A;
+  if (p.gw) p.gw[i] = B;
+}
+
+// ---- host ------------------------------------------------------------------------------------
+
+// Vector width and the cut of [S, C] into blocks: a block covers up to 256 vectors of a row and as
+// many rows at once as its threads allow; S is cut into enough chunks to fill the GPU, none
+// shorter than 64 rows, so that the partial sums stay below a sixteenth of what is read.
+void plan(NormArgs* p, int V) {
+  const int vecs = p->C / V;
+  p->cl = vecs < kThreads ? vecs : kThreads;
+  p->cblocks = static_cast<int>(dpk_cdiv(vecs, p->cl));
+  const int step = kThreads / p->cl;
+  const int64_t least = static_cast<int64_t>(step) * kRows > 64 ? static_cast<int64_t>(step) * kRows : 64;
+  int64_t J = dpk_cdiv(kWantBlocks, p->n * p->cblocks);
+  const int64_t most = dpk_cdiv(p->S, least);
+  if (J > most) J = most;
+  if (J < 1) J = 1;
+  p->chunk = dpk_cdiv(p->S, J);
+  p->J = static_cast<int>(dpk_cdiv(p->S, p->chunk));
+}
+
+int width_of(const NormArgs& p, int dtype) {
+  for (int V = dtype == DPK_BF16 ? 8 : 4; V > 1; V /= 2) {
+    const size_t al = dpk_elsize(dtype) * V;
+    if (p.C % V == 0 && dpk_aligned(p.x, al) && dpk_aligned(p.dy, al) && dpk_aligned(p.y, al)) return V;
+  }
+  return 1;
+}
+
+size_t part_bytes(int64_t n, int64_t S, int64_t C) {
+  size_t most = 0;
+  for (int V = 1; V <= 8; V *= 2) {  // whichever width the pointers allow
+    if (C % V) break;
+    NormArgs p = {};
+    p.n = n, p.S = S, p.C = static_cast<int>(C);
+    plan(&p, V);
+    const size_t need = static_cast<size_t>(n) * p.J * C * sizeof(float2);
+    if (need > most) most = need;
+  }
+  return dpk_align_up(most, 256);
+}
+size_t group_bytes(int64_t n, int64_t S, int64_t G, int per_position) {
+  return dpk_align_up(static_cast<size_t>(n) * (per_position ? S : 1) * G * sizeof(float2), 256);
+}
+
+int check_common(const char* fn, const NormArgs& p, int dtype, int param_dtype, int64_t C, int64_t G, int per_position,
+                 const void* ws, size_t ws_bytes, bool* nothing) {
+  *nothing = false;
+  DPK_REQUIRE(p.n >= 0 && p.S >= 0 && C >= 1 && G >= 1, DPK_E_SHAPE, "%s: bad size (n=%lld S=%lld C=%lld groups=%lld)", fn,
+              (long long)p.n, (long long)p.S, (long long)C, (long long)G);
+  DPK_REQUIRE(C % G == 0, DPK_E_SHAPE, "%s: %lld channels do not divide into %lld groups", fn, (long long)C, (long long)G);
+  DPK_REQUIRE(C <= (1 << 24) && p.n < (1LL << 31) && p.S < (1LL << 40), DPK_E_SHAPE, "%s: too large", fn);
+  DPK_REQUIRE(dpk_dtype_ok(dtype) && dpk_dtype_ok(param_dtype), DPK_E_DTYPE, "%s: dtype %d / %d not supported", fn, dtype,
+              param_dtype);
+  DPK_REQUIRE(p.act >= DPK_ACT_NONE && p.act <= DPK_ACT_GELU, DPK_E_ARG, "%s: unknown activation %d", fn, p.act);
+  DPK_REQUIRE(per_position == 0 || per_position == 1, DPK_E_ARG, "%s: per_position must be 0 or 1", fn);
+  DPK_REQUIRE(p.eps >= 0.f, DPK_E_ARG, "%s: eps must not be negative", fn);
+  if (p.n == 0 || p.S == 0) {
+    *nothing = true;
+    return DPK_OK;
+  }
+  const size_t es = dpk_elsize(dtype), ps = dpk_elsize(param_dtype);
+  DPK_REQUIRE(p.x && p.y, DPK_E_ARG, "%s: a tensor is NULL", fn);
+  DPK_REQUIRE(dpk_aligned(p.x, es) && dpk_aligned(p.y, es) && dpk_aligned(p.dy, es) && dpk_aligned(p.w, ps) &&
+                  dpk_aligned(p.b, ps) && dpk_aligned(p.gw, 4) && dpk_aligned(p.gb, 4) && dpk_aligned(p.stats, 8),
+              DPK_E_ALIGN, "%s: a tensor is not aligned to its element size", fn);
+  DPK_REQUIRE(p.n * G <= DPK_MAX_GRID_X && (!per_position || dpk_cdiv(p.n * p.S * G, 4) <= DPK_MAX_GRID_X), DPK_E_SHAPE,
+              "%s: too many groups", fn);
+  const size_t need = dpk_group_norm_act_workspace_bytes(p.n, p.S, C, G, per_position);
+  DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
+  DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
+  return DPK_OK;
+}
+
+// Calls body(T{}, integral_constant<V>) for the tensor's type and width.
+template <typename F>
+void by_width(int dtype, int V, F&& body) {
+  if (dtype == DPK_BF16) {
+    if (V == 8) body(bf16_t(), std::integral_constant<int, 8>());
+    else if (V == 4) body(bf16_t(), std::integral_constant<int, 4>());
+    else if (V == 2) body(bf16_t(), std::integral_constant<int, 2>());
+    else body(bf16_t(), std::integral_constant<int, 1>());
+  } else {
+    if (V == 4) body(float(), std::integral_constant<int, 4>());
+    else if (V == 2) body(float(), std::integral_constant<int, 2>());
+    else body(float(), std::integral_constant<int, 1>());
+  }
+}
+
+}  // namespace
+
+extern "C" size_t dpk_group_norm_act_workspace_bytes(int64_t n, int64_t S, int64_t C, int64_t groups, int per_position) {
+  if (n <= 0 || S <= 0 || C <= 0 || groups <= 0) return 0;
+  return part_bytes(n, S, C) + group_bytes(n, S, groups, per_position);
+}
+
+extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, const void* bias, int param_dtype, void* y,
+                                  float* stats, int64_t n, int64_t S, int64_t C, int64_t groups, float eps, int act,
+                                  int per_position, void* ws, size_t ws_bytes, dpk_stream_t stream) {
+  const char* fn = "dpk_group_norm_act";
+  NormArgs p = {};
+  p.x = x, p.w = weight, p.b = bias, p.y = y, p.stats = reinterpret_cast<float2*>(stats);
+  p.n = n, p.S = S, p.act = act, p.eps = eps, p.param_bf16 = param_dtype == DPK_BF16;
+  bool nothing;
+  if (int rc = check_common(fn, p, dtype, param_dtype, C, groups, per_position, ws, ws_bytes, &nothing)) return rc;
+  if (nothing) return DPK_OK;
+  DPK_REQUIRE(stats || per_position, DPK_E_ARG, "%s: stats is NULL", fn);
+  p.C = static_cast<int>(C), p.G = static_cast<int>(groups), p.Cg = p.C / p.G;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (per_position) {
+    const unsigned grid = static_cast<unsigned>(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE));
+    if (dtype == DPK_BF16) hipLaunchKernelGGL((position_kernel<bf16_t, false>), dim3(grid), dim3(kThreads), 0, s, p);
+    else hipLaunchKernelGGL((position_kernel<float, false>), dim3(grid), dim3(kThreads), 0, s, p);
+  } else {
+    const int V = width_of(p, dtype);
+    plan(&p, V);
+    p.part = static_cast<float2*>(ws);
+    const int64_t blocks = n * p.cblocks * p.J;
+    DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    by_width(dtype, V, [&](auto t, auto v) {
+      hipLaunchKernelGGL((sample_stat_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0, s, p);
+    });
+    hipLaunchKernelGGL(sample_stat_merge_kernel, dim3(static_cast<unsigned>(n * groups)), dim3(kThreads), 0, s, p);
+    by_width(dtype, V, [&](auto t, auto v) {
+      hipLaunchKernelGGL((sample_apply_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0, s, p);
+    });
+  }
+  DPK_LAUNCH_CHECK(fn);
+  return DPK_OK;
+}
+
+extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, int dtype, const void* weight,
+                                           const void* bias, int param_dtype, const float* stats, void* grad_x,
+                                           float* grad_weight, float* grad_bias, int64_t n, int64_t S, int64_t C,
+                                           int64_t groups, float eps, int act, int per_position, void* ws, size_t ws_bytes,
+                                           dpk_stream_t stream) {
+  const char* fn = "dpk_group_norm_act_backward";
+  NormArgs p = {};
+  p.x = x, p.dy = grad_out, p.w = weight, p.b = bias, p.y = grad_x;
+  p.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+  p.gw = grad_weight, p.gb = grad_bias;
+  p.n = n, p.S = S, p.act = act, p.eps = eps, p.param_bf16 = param_dtype == DPK_BF16;
+  bool nothing;
+  if (int rc = check_common(fn, p, dtype, param_dtype, C, groups, per_position, ws, ws_bytes, &nothing)) return rc;
+  if (nothing) return DPK_OK;
+  DPK_REQUIRE(grad_out, DPK_E_ARG, "%s: grad_out is NULL", fn);
+  DPK_REQUIRE(stats || per_position, DPK_E_ARG, "%s: stats is NULL", fn);
+  p.C = static_cast<int>(C), p.G = static_cast<int>(groups), p.Cg = p.C / p.G;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int V = width_of(p, dtype);
+  plan(&p, V);
+  const int64_t blocks = n * p.cblocks * p.J;
+  DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  p.part = static_cast<float2*>(ws);
+  float2* groups_ws = reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(n, S, C));
+  if (per_position) {
+    p.stats = groups_ws;
+    const unsigned waves = static_cast<unsigned>(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE));
+    if (dtype == DPK_BF16) hipLaunchKernelGGL((position_kernel<bf16_t, true>), dim3(waves), dim3(kThreads), 0, s, p);
+    else hipLaunchKernelGGL((position_kernel<float, true>), dim3(waves), dim3(kThreads), 0, s, p);
+    if (p.gw || p.gb) {
+      by_width(dtype, V, [&](auto t, auto v) {
+        hipLaunchKernelGGL((channel_sums_kernel<decltype(t), decltype(v)::value, true>), grid, dim3(kThreads), 0, s, p);
+      });
+      hipLaunchKernelGGL(chunk_merge_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * C, kThreads))), dim3(kThreads), 0, s, p);
+    }
+  } else {
+    p.sums = groups_ws;
+    by_width(dtype, V, [&](auto t, auto v) {
+      hipLaunchKernelGGL((channel_sums_kernel<decltype(t), decltype(v)::value, false>), grid, dim3(kThreads), 0, s, p);
+    });
+    hipLaunchKernelGGL(sample_grad_merge_kernel, dim3(static_cast<unsigned>(n * groups)), dim3(kThreads), 0, s, p);
+    by_width(dtype, V, [&](auto t, auto v) {
+      hipLaunchKernelGGL((sample_dx_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0, s, p);
+    });
+  }
+  DPK_LAUNCH_CHECK(fn);
+  return DPK_OK;
+}

@@ -1042,6 +1042,112 @@ def gated_scan_step(gates: torch.Tensor, decay: torch.Tensor, state: torch.Tenso
     return out
 
 
+# ---- group norm with an activation, channels last ------------------------------------------
+def _norm_act_args(x, num_groups, weight, bias, eps, activation):
+    dev = _need_gpu(x, weight, bias)
+    if x.dim() < 2:
+        raise ValueError(f"x must be [n, *, C], got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if num_groups < 1 or C < 1 or C % num_groups:
+        raise ValueError(f"{C} channels do not divide into {num_groups} groups")
+    if activation not in _lib.DPK_ACT:
+        raise ValueError(f"activation must be one of {sorted(_lib.DPK_ACT)}, got {activation!r}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    _code(x)
+    params = [p for p in (weight, bias) if p is not None]
+    for p in params:
+        if tuple(p.shape) != (C,):
+            raise ValueError(f"weight and bias must have shape ({C},), got {tuple(p.shape)}")
+    if len(params) == 2 and weight.dtype != bias.dtype:
+        raise ValueError(f"weight and bias differ in dtype: {weight.dtype} and {bias.dtype}")
+    weight, bias = (None if p is None else _dense(p) for p in (weight, bias))
+    return dev, weight, bias, (_code(params[0]) if params else DPK_F32)
+
+
+def group_norm_act(
+    x: torch.Tensor,
+    num_groups: int,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    eps: float = 1e-5,
+    activation: str = "none",
+    per_position: bool = False,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``act(weight * group_norm(x) + bias)`` of a channels-last ``[n, *, C]`` tensor, ``act`` one of
+    none, relu, silu and gelu (erf). The statistics of a group of ``C / num_groups`` neighbouring
+    channels run over all positions of the sample (``nn.GroupNorm``), or with ``per_position`` over
+    each position alone (the heads of a token). Returns ``(y, stats)``; ``stats`` (None with
+    ``per_position``) goes to :func:`group_norm_act_backward`."""
+    dev, weight, bias, pcode = _norm_act_args(x, num_groups, weight, bias, eps, activation)
+    x = _dense(x)
+    n, C = x.shape[0], x.shape[-1]
+    S = math.prod(x.shape[1:-1])
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = None if per_position else torch.empty((n, num_groups, 2), dtype=torch.float32, device=dev)
+    if n == 0 or S == 0:
+        return y, stats
+    L = lib()
+    ws, wsb = _ws(L.dpk_group_norm_act_workspace_bytes(n, S, C, num_groups, int(bool(per_position))), dev)
+    with _on(dev), _timed("group_norm_act", dev):
+        check(
+            "dpk_group_norm_act",
+            L.dpk_group_norm_act(
+                _ptr(x), _code(x), _ptr(weight), _ptr(bias), pcode, _ptr(y), _ptr(stats), n, S, C, num_groups, float(eps),
+                _lib.DPK_ACT[activation], int(bool(per_position)), _ptr(ws), wsb, _stream(dev),
+            ),
+        )
+    return y, stats
+
+
+def group_norm_act_backward(
+    x: torch.Tensor,
+    grad_out: torch.Tensor,
+    stats: Optional[torch.Tensor],
+    num_groups: int,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    eps: float = 1e-5,
+    activation: str = "none",
+    per_position: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of :func:`group_norm_act`: ``(grad_x, grad_weight [n, C], grad_bias [n, C])``. The
+    last two (float32) are the per-sample gradients; the pass over ``x`` and ``grad_out`` that the
+    input gradient needs has them on the way."""
+    dev, weight, bias, pcode = _norm_act_args(x, num_groups, weight, bias, eps, activation)
+    _need_gpu(x, grad_out, stats)
+    if grad_out.shape != x.shape:
+        raise ValueError(f"grad_out must be {tuple(x.shape)}, got {tuple(grad_out.shape)}")
+    if grad_out.dtype != x.dtype:
+        grad_out = grad_out.to(x.dtype)
+    x, grad_out = _dense(x), _dense(grad_out)
+    n, C = x.shape[0], x.shape[-1]
+    S = math.prod(x.shape[1:-1])
+    if not per_position:
+        if stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (n, num_groups, 2):
+            raise ValueError(f"stats must be what group_norm_act returned, float32 {(n, num_groups, 2)}")
+        stats = _dense(stats)
+    else:
+        stats = None
+    grad_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if n == 0 or S == 0:
+        return grad_x, torch.zeros((n, C), device=dev), torch.zeros((n, C), device=dev)
+    grad_w = torch.empty((n, C), dtype=torch.float32, device=dev)
+    grad_b = torch.empty((n, C), dtype=torch.float32, device=dev)
+    L = lib()
+    ws, wsb = _ws(L.dpk_group_norm_act_workspace_bytes(n, S, C, num_groups, int(bool(per_position))), dev)
+    with _on(dev), _timed("group_norm_act_backward", dev):
+        check(
+            "dpk_group_norm_act_backward",
+            L.dpk_group_norm_act_backward(
+                _ptr(x), _ptr(grad_out), _code(x), _ptr(weight), _ptr(bias), pcode, _ptr(stats), _ptr(grad_x), _ptr(grad_w),
+                _ptr(grad_b), n, S, C, num_groups, float(eps), _lib.DPK_ACT[activation], int(bool(per_position)),
+                _ptr(ws), wsb, _stream(dev),
+            ),
+        )
+    return grad_x, grad_w, grad_b
+
+
 # ---- optimizer: norms, clip factor, clip-weighted sum, noise ---------------------------
 def _flat2d(gs: torch.Tensor) -> torch.Tensor:
     g = _dense(gs)
