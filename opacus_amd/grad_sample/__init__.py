@@ -30,6 +30,7 @@ from .group_norm import compute_group_norm_grad_sample  # noqa: E402
 from .instance_norm import compute_instance_norm_grad_sample  # noqa: E402
 from .layer_norm import compute_layer_norm_grad_sample  # noqa: E402
 from .linear import compute_linear_grad_sample, compute_linear_norm_sample  # noqa: E402
+from .param_rows import compute_gated_scan_grad_sample, compute_norm_act_grad_sample  # noqa: E402
 from .rms_norm import compute_rms_norm_grad_sample  # noqa: E402
 
 __all__ = [

@@ -247,9 +247,19 @@ class GradSampleHooks(AbstractGradSampleHooks):
     def add_hooks(self, *, loss_reduction: str = "mean", batch_first: bool = True, force_functorch: bool = False) -> None:
         if hasattr(self._module, "autograd_grad_sample_hooks"):
             raise ValueError("Trying to add hooks twice to the same model")
+        for module in self.iterate_submodules(self._module):
+            if force_functorch or self._get_module_type(module) not in self.GRAD_SAMPLERS:
+                for m in module.modules():
+                    if getattr(m, "per_sample_rows", False):
+                        raise NotImplementedError(
+                            f"{type(m).__name__} has no functorch path: its per-sample gradients come from its own "
+                            "backward kernel (grad_sample_mode='hooks' or 'ghost', outside layers without a sampler)"
+                        )
         self._module.autograd_grad_sample_hooks = []
         self.autograd_grad_sample_hooks = self._module.autograd_grad_sample_hooks
         for module in self.iterate_submodules(self._module):
+            if getattr(module, "per_sample_rows", False):
+                module.__dict__["_dpk_rows_hooked"] = True
             if force_functorch or self._get_module_type(module) not in self.GRAD_SAMPLERS:
                 prepare_layer(module, batch_first=batch_first)
             elif not self.autograd_weight_grads:
@@ -299,11 +309,16 @@ class GradSampleHooks(AbstractGradSampleHooks):
         an extra autograd node per call, which is what a small launch-bound model pays for
         in every step, and it tolerates an in-place op on the output."""
         d = module.__dict__
+        rows = d.pop("_dpk_param_rows", None)
         pending = len(d.get("activations", ()))
         self.capture_activations_hook(module, forward_input, forward_output)
         if len(d.get("activations", ())) == pending:
             return  # nothing captured: eval mode, no grad, hooks disabled, frozen module
         out = forward_output if isinstance(forward_output, torch.Tensor) else forward_output[0]
+        if rows is not None:
+            # the layer's own backward kernel leaves the per-sample gradients: they arrive as the
+            # gradient of its parameters' rows (layers/param_rows.py), which the sampler gets as backprops
+            out = rows
         tapped = d.pop("_dpk_at_start", False) and isinstance(forward_output, torch.Tensor)
         if tapped and not out.requires_grad:
             out = _GradTap.apply(out, self._tap_anchor)
@@ -330,6 +345,9 @@ class GradSampleHooks(AbstractGradSampleHooks):
             delattr(self, "autograd_grad_sample_hooks")
             if hasattr(self._module, "autograd_grad_sample_hooks"):
                 delattr(self._module, "autograd_grad_sample_hooks")
+        for module in self._module.modules():
+            module.__dict__.pop("_dpk_rows_hooked", None)
+            module.__dict__.pop("_dpk_param_rows", None)
         for _, module in trainable_modules(self._module):
             if hasattr(module, "ft_compute_sample_grad"):
                 delattr(module, "ft_compute_sample_grad")
@@ -459,7 +477,8 @@ class GradSampleHooks(AbstractGradSampleHooks):
             raise ValueError(f"No activations detected for {type(module)}, run forward after add_hooks(model)")
         # the recurrent layers feed their RNNLinear batch first whatever the model's layout
         # (grad_sample_module.py:391)
-        batch_dim = 0 if batch_first or getattr(module, "stack_uses", False) else 1
+        always_first = getattr(module, "stack_uses", False) or getattr(module, "per_sample_rows", False)
+        batch_dim = 0 if batch_first or always_first else 1
         if "max_batch_len" not in module.__dict__:
             module.__dict__["max_batch_len"] = _get_batch_size(module=module, batch_dim=batch_dim)
         activations = module.activations.pop()

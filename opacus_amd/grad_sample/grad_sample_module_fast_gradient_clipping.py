@@ -155,7 +155,11 @@ class GradSampleHooksFastGradientClipping(GradSampleHooks):
         requires grad (or, where such an output is not a single tensor, their parameters),
         and inputs that are leaves requiring grad."""
         tensors = [t for t in forward_input if isinstance(t, torch.Tensor)]
-        if not any(t.requires_grad for t in tensors):
+        if getattr(module, "per_sample_rows", False):
+            # the hook listens to the parameters' rows, so the pass has to reach the parameters
+            for _, p in trainable_parameters(module):
+                self._first_pass_leaves[id(p)] = (p, None, module)
+        elif not any(t.requires_grad for t in tensors):
             if isinstance(forward_output, torch.Tensor) and forward_output.requires_grad:
                 # kept with its version: an in-place op on it later moves the tensor to
                 # another node of the graph, and the module's parameters are asked for instead
