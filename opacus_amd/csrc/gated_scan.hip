@@ -4,11 +4,11 @@
 //   rho = sigma(r);  L = -softplus(lam) rho;  a = exp(L);  u = sqrt(1 - a^2) sigma(i) x
 //   h_t = a_t h_{t-1} + u_t,   out_t = h_t
 //
-// The recurrence is a composition of affine maps h -> A h + B, so T is cut at will: every thread
-// runs K positions of its channels in registers, the 16 time groups of a block exchange their
-// (A, B) through LDS and fold them in order, and where the batch has too few rows to fill the
-// GPU, T is also cut into segments whose (A, B) a first launch leaves in the workspace. Every fold runs in
-// position order: the same inputs give the same bits.
+// The recurrence is a composition of affine maps h -> A h + B, so T is cut at will. A block takes one
+// tile of positions for 16 * V channels of a sample: every thread runs K positions of its channels in
+// registers, the 16 time groups exchange their (A, B) through LDS, and the tiles of a row pass
+// the state on in one launch (see "the chain" below), so every input is read once and every output
+// written once. What is folded, and in which order, depends on sizes alone: the same bits on every run.
 //
 // Backward: g_t = dy_t + a_{t+1} g_{t+1} runs the same maps the other way (same A, other B), and
 //   q = 1 - a,  m = sqrt(q (1 + a)),  kappa = -L / m,  s = sigma(i)
@@ -25,47 +25,164 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCL = 16;                  // lanes across channels
+constexpr int kCL = 32;                  // lanes across channels
 constexpr int kTG = kThreads / kCL;      // time groups of a block
 constexpr int kChunk = DPK_SCAN_CHUNK;   // positions between kept states
-constexpr int kFwdK = 8;                 // positions per thread and tile
-constexpr int kBwdK = 4;
+constexpr int kFwdK = 16;                // positions per thread
+constexpr int kBwdK = 8;
 constexpr int kFwdTile = kTG * kFwdK;    // 128
 constexpr int kBwdTile = kTG * kBwdK;    // 64
-static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0, "a backward tile starts at a kept state");
-// Blocks wanted before T is left whole: four per CU of the MI355X.
-constexpr int64_t kWantBlocks = 1024;
-constexpr int kMaxSegments = 64;
+static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0 && kChunk % kFwdK == 0, "tiles start at kept states");
+// Byte offsets inside a tile are 32 bits wide.
+constexpr int64_t kMaxStride = (1LL << 31) / (kFwdTile * 4) - 1;
 
-// softplus(v) = max(v, 0) + log1p(exp(-|v|))
-__device__ __forceinline__ float softplus_f(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
+// softplus(v) = max(v, 0) + log1p(exp(-|v|)), with log1p(e) = log(1 + e) * e / ((1 + e) - 1): the
+// quotient corrects what the rounding of 1 + e did, so the result keeps its relative accuracy as
+// e vanishes. Hardware exp2, log2 and reciprocal.
+__device__ __forceinline__ float softplus_f(float v) {
+  const float e = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2e), u = 1.0f + e, d = u - 1.0f;
+  const float l = d > 0.f ? __builtin_amdgcn_logf(u) * 0.69314718055994531f * (e * __builtin_amdgcn_rcpf(d)) : e;
+  return fmaxf(v, 0.f) + l;
+}
 // sigma(v) / softplus(v); 1 in the limit v -> -inf, where both are exp(v)
 __device__ __forceinline__ float decay_ratio(float v) {
   const float sp = softplus_f(v);
-  return sp > 0.f ? (1.0f / (1.0f + expf(-v))) / sp : 1.0f;
+  return sp > 0.f ? sigmoid_f(v) / sp : 1.0f;
 }
 
-// a = exp(L) and q = 1 - a for L <= 0, each to its own relative accuracy: q from its series
-// -L (1 + L/2 + L^2/6 + ...) while |L| < 0.35 (the first dropped term is below 2e-8), from a beyond.
-// A layer starts out with every L in the series' range, so the exponential is behind a branch
-// that a wave takes only if one of its lanes needs it.
-__device__ __forceinline__ void decay_of(float L, float& a, float& q) {
-  float p = fmaf(L, 1.0f / 5040.0f, 1.0f / 720.0f);
-  p = fmaf(L, p, 1.0f / 120.0f);
-  p = fmaf(L, p, 1.0f / 24.0f);
-  p = fmaf(L, p, 1.0f / 6.0f);
-  p = fmaf(L, p, 0.5f);
-  p = fmaf(L, p, 1.0f);
-  q = -L * p;
-  a = 1.0f - q;
-  if (!(L > -0.35f)) {
-    a = __builtin_amdgcn_exp2f(L * kLog2e);
-    q = 1.0f - a;
+// For the decay gates of one position: L = -softplus(lam) sigma(r), a = exp(L) and q = 1 - a, each
+// to its own relative accuracy: q = -L P(L) while L > -0.7, P the degree-5 polynomial nearest to
+// (exp(L) - 1) / L there (1e-8 of it off; found by Remez exchange), q = 1 - a beyond. A layer starts out
+// with every L in the polynomial's range; the exponentials are behind one branch for the V elements,
+// which a wave takes only if one of its lanes needs it.
+template <int V>
+__device__ __forceinline__ void decay_of(const float (&L)[V], float (&a)[V], float (&q)[V]) {
+  float low = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    low = fminf(low, L[j]);
+    float p = fmaf(L[j], 0.0010301340371370316f, 0.008062456734478474f);
+    p = fmaf(L[j], p, 0.04156935214996338f);
+    p = fmaf(L[j], p, 0.16665059328079224f);
+    p = fmaf(L[j], p, 0.4999990165233612f);
+    p = fmaf(L[j], p, 1.0f);
+    q[j] = -L[j] * p;
+    a[j] = 1.0f - q[j];
+  }
+  if (__any(low <= -0.7f)) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float e = __builtin_amdgcn_exp2f(L[j] * kLog2e);
+      const bool far = L[j] <= -0.7f;
+      a[j] = far ? e : a[j];
+      q[j] = far ? 1.0f - e : q[j];
+    }
   }
 }
-// 1 / sqrt(1 - a^2) from q. A q of zero gives a finite factor, so that m = (1 - a^2) * this and
+// 1 / sqrt(1 - a^2) from 1 - a^2. A zero gives a finite factor, so that m = (1 - a^2) * this and
 // kappa = -L * this are zero there.
 __device__ __forceinline__ float inv_scale(float q2) { return __builtin_amdgcn_rsqf(fmaxf(q2, 1e-37f)); }
+
+// ---- the chain: tiles of one row hand the state on within a launch -----------------------------
+//
+// A row is 16 * V channels of one sample; its tiles are numbered by a ticket each block draws when
+// it starts, so a block only ever waits for blocks that are already running and that never wait
+// for it. Every tile but the row's last publishes its (A, B); 16 tiles form a run, and the last
+// tile of a run publishes the state after it. A tile waits for the (A, B) of the tiles before it in its
+// run and for the state the run started from, and folds them in position order. What it adds up
+// never depends on timing, so the bits repeat; the serial part of a row is one hop per run.
+// A word is 64 bits, stored and read whole at agent scope (the XCDs' L2s are not coherent), with
+// the pattern kEmpty in its low half until it is written; a NaN is published as the usual quiet one.
+constexpr int kRun = 16;
+constexpr uint32_t kEmpty = 0xffffffffu;
+
+struct Chain {
+  uint32_t* tickets;  // [rows], zero at the start
+  uint64_t* maps;     // [rows, tiles, W]
+  uint64_t* states;   // [rows, runs, W]
+  int64_t rows;
+  int tiles, runs;
+};
+
+__device__ __forceinline__ void publish(uint64_t* w, float a, float b) {
+  const uint32_t lo = a != a ? 0x7fc00000u : __float_as_uint(a);
+  __hip_atomic_store(w, (static_cast<uint64_t>(__float_as_uint(b)) << 32) | lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <int V>
+__device__ __forceinline__ void await(const uint64_t* w, float* a, float* b) {
+  uint64_t v[V];
+  bool there;
+  do {
+    there = true;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      v[j] = __hip_atomic_load(w + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      there = there && static_cast<uint32_t>(v[j]) != kEmpty;
+    }
+    if (!there) __builtin_amdgcn_s_sleep(1);
+  } while (!there);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    a[j] = __uint_as_float(static_cast<uint32_t>(v[j]));
+    b[j] = __uint_as_float(static_cast<uint32_t>(v[j] >> 32));
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void chain_clear_kernel(uint32_t* tickets, int64_t rows, uint64_t* words, int64_t count) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < count; i += step) words[i] = ~0ull;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < rows; i += step) tickets[i] = 0;
+}
+
+// This block's tile number in its row, in the order of the chain.
+__device__ __forceinline__ int draw_tile(const Chain& ch, int64_t row, int* lds) {
+  if (ch.tiles == 1) return 0;
+  if (threadIdx.x == 0) *lds = static_cast<int>(__hip_atomic_fetch_add(ch.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  __syncthreads();
+  return *lds;
+}
+
+// The state that enters tile `t` of the row whose own map is (TA, TB) and whose first state is `in`
+// (which receives it). All threads call it; lds: [2][kRun][W] and [W] floats nobody else uses.
+template <int V>
+__device__ __forceinline__ void through_chain(const Chain& ch, int64_t row, int t, int cl, int tg, const float (&TA)[V],
+                                              const float (&TB)[V], float (&in)[V], float* lds_m, float* lds_s) {
+  constexpr int W = kCL * V;
+  const int run = t / kRun, k = t - run * kRun;
+  const bool more = t + 1 < ch.tiles;
+  if (more && k + 1 < kRun && tg == 0) {
+    uint64_t* w = ch.maps + (row * ch.tiles + t) * W + cl * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) publish(w + j, TA[j], TB[j]);
+  }
+  if (t > 0) {
+    float x[V], y[V];
+    for (int g = tg; g < k; g += kTG) {
+      await<V>(ch.maps + (row * ch.tiles + run * kRun + g) * W + cl * V, x, y);
+#pragma unroll
+      for (int j = 0; j < V; ++j) lds_m[g * W + cl * V + j] = x[j], lds_m[(kRun + g) * W + cl * V + j] = y[j];
+    }
+    if (tg == kTG - 1 && run > 0) {
+      await<V>(ch.states + (row * ch.runs + run) * W + cl * V, x, y);
+#pragma unroll
+      for (int j = 0; j < V; ++j) lds_s[cl * V + j] = y[j];
+    }
+    __syncthreads();
+    if (run > 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) in[j] = lds_s[cl * V + j];
+    }
+    for (int g = 0; g < k; ++g) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) in[j] = fmaf(lds_m[g * W + cl * V + j], in[j], lds_m[(kRun + g) * W + cl * V + j]);
+    }
+  }
+  if (more && k + 1 == kRun && tg == 0) {
+    uint64_t* w = ch.states + (row * ch.runs + run + 1) * W + cl * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) publish(w + j, 0.f, fmaf(TA[j], in[j], TB[j]));
+  }
+}
 
 struct ScanArgs {
   const void* gates;
@@ -75,12 +192,9 @@ struct ScanArgs {
   void* out;
   float* last;
   float* kept;             // [n, ceil(T/chunk), D] or null
-  float* sum_a;            // [S,n,D] summaries of the segments
-  float* sum_b;
   int64_t n, T, D, sn, st;
   int decay_bf16, reverse;
-  int S;                   // segments of T
-  int64_t seg;             // positions of a segment, a multiple of the tile
+  Chain ch;
 };
 
 struct ScanBwdArgs {
@@ -92,13 +206,10 @@ struct ScanBwdArgs {
   const float* dlast;      // [n,D] or null
   void* dgates;            // [n,T,3D]
   float* dstate;           // [n,D] or null
-  float* dlam;             // [S,n,D]: the rows themselves when S == 1
-  float* sum_a;
-  float* sum_b;
+  float* dlam;             // [tiles,n,D] (the result itself if there is one tile) or null
   int64_t n, T, D, sn, st;
   int decay_bf16, reverse;
-  int S;
-  int64_t seg;
+  Chain ch;
 };
 
 template <int V>
@@ -114,373 +225,357 @@ __device__ __forceinline__ int64_t live_length(const int64_t* lengths, int64_t b
   return l < 0 ? 0 : (l < T ? l : T);
 }
 
-// One block: 16 * V channels of one sample, one segment of T, walked tile by tile.
-// SUMMARY: only (A, B) of the segment are wanted.
-template <typename T, int V, bool SUMMARY>
+// The positions of one tile, in the order of the scan: local position l is position
+// (reverse ? T - 1 - s0 - l : s0 + l); those of [lo, hi) are live, those below count exist. `at(l)` is the
+// element offset of l from the tile's lowest position at the given stride.
+struct Tile {
+  int64_t low;  // lowest position
+  int lo, hi, count;
+  bool reverse;
+  __device__ __forceinline__ int at(int l, int stride) const { return (reverse ? count - 1 - l : l) * stride; }
+};
+template <typename T, int V>
+__device__ __forceinline__ typename vec_io<T, V>::raw load_at(const T* base, uint32_t bytes) {
+  return vec_io<T, V>::load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + bytes));
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_at(T* base, uint32_t bytes, const float* v) {
+  vec_io<T, V>::store(reinterpret_cast<T*>(reinterpret_cast<char*>(base) + bytes), v);
+}
+template <int SIZE>
+__device__ __forceinline__ Tile tile_of(int64_t T, int64_t len, int64_t s0, int reverse) {
+  Tile t;
+  t.reverse = reverse != 0;
+  t.count = static_cast<int>(T - s0 < SIZE ? T - s0 : SIZE);
+  t.low = t.reverse ? T - s0 - t.count : s0;
+  // live positions are those below len: in scan order a prefix, or in reverse a suffix
+  int64_t n = len - t.low;
+  n = n < 0 ? 0 : (n < t.count ? n : t.count);
+  t.lo = t.reverse ? t.count - static_cast<int>(n) : 0;
+  t.hi = t.reverse ? t.count : static_cast<int>(n);
+  return t;
+}
+
+// prefix = the composition of the groups before tg, total = of all kTG, in the order of the scan
+// (BACK: from the last group to the first). The wave's own groups are the only ones at which
+// lanes differ, so the rest is folded without selects.
+template <int V, bool BACK>
+__device__ __forceinline__ void fold_groups(const float (*la)[kCL * V], const float (*lb)[kCL * V], int cl, int tg,
+                                            float (&PA)[V], float (&PB)[V], float (&TA)[V], float (&TB)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) TA[j] = PA[j] = 1.f, TB[j] = PB[j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kTG; ++i) {
+    const int g = BACK ? kTG - 1 - i : i;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (g == tg) PA[j] = TA[j], PB[j] = TB[j];
+      const float ga = la[g][cl * V + j];
+      TB[j] = fmaf(ga, TB[j], lb[g][cl * V + j]);
+      TA[j] *= ga;
+    }
+  }
+}
+
+// FULL: every position and channel of the tile is live.
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
+                                         float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float* lds_m, float* lds_s) {
+  typedef vec_io<T, V> io;
+  constexpr int W = kCL * V, K = kFwdK, E = sizeof(T);
+  const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
+  const int cw = cl * V, c = static_cast<int>(cb) * W + cw;
+  const bool on = FULL || c < p.D;
+  const int D = static_cast<int>(p.D), st = static_cast<int>(p.st);
+  const T* gx = static_cast<const T*>(p.gates) + b * p.sn + tl.low * p.st + cb * W;
+  const T *gr = gx + D, *gi = gr + D;
+
+  typename io::raw rx[K], rr[K], ri[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int l = tg * K + k;
+    if (!FULL) rx[k] = rr[k] = ri[k] = typename io::raw();
+    if (FULL || (on && l >= tl.lo && l < tl.hi)) {
+      const uint32_t q = tl.at(l, st * E) + cw * E;
+      rx[k] = load_at<T, V>(gx, q);
+      rr[k] = load_at<T, V>(gr, q);
+      ri[k] = load_at<T, V>(gi, q);
+    }
+  }
+  const int64_t row = b * p.D + c;
+  float sp[V], h[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sp[j] = h[j] = 0.f;
+  if (on) {
+    load_decay<V>(p.decay, p.decay_bf16, c, sp);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sp[j] = softplus_f(sp[j]);
+    if (p.state && t < kRun) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[j] = p.state[row + j];
+    }
+  }
+  float a[K][V], u[K][V], A[V], B[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool live = FULL || (tg * K + k >= tl.lo && tg * K + k < tl.hi);
+    float L[V], q[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) L[j] = live ? -sp[j] * sigmoid_f(io::get(rr[k], j)) : 0.f;
+    decay_of<V>(L, a[k], q);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float m = __builtin_amdgcn_sqrtf(fmaf(q[j], a[k][j], q[j]));
+      u[k][j] = m * sigmoid_f(io::get(ri[k], j)) * io::get(rx[k], j);
+      A[j] *= a[k][j];
+      B[j] = fmaf(a[k][j], B[j], u[k][j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) lds_a[tg][cw + j] = A[j], lds_b[tg][cw + j] = B[j];
+  __syncthreads();
+  float TA[V], TB[V], PA[V], PB[V];
+  fold_groups<V, false>(lds_a, lds_b, cl, tg, PA, PB, TA, TB);
+  through_chain<V>(p.ch, r, t, cl, tg, TA, TB, h, lds_m, lds_s);
+  if (on && tg == 0 && t + 1 == p.ch.tiles) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.last[row + j] = fmaf(TA[j], h[j], TB[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) h[j] = fmaf(PA[j], h[j], PB[j]);
+  if (!on || tg * K >= tl.count) return;
+  if (p.kept && (tg * K) % kChunk == 0) {
+    const int64_t s = static_cast<int64_t>(t) * kFwdTile + tg * K;
+    vec_io<float, V>::store(p.kept + (b * ((p.T + kChunk - 1) / kChunk) + s / kChunk) * p.D + c, h);
+  }
+  T* out = static_cast<T*>(p.out) + (b * p.T + tl.low) * p.D + cb * W;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int l = tg * K + k;
+    const bool live = FULL || (l >= tl.lo && l < tl.hi);
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      h[j] = fmaf(a[k][j], h[j], u[k][j]);
+      o[j] = live ? h[j] : 0.f;
+    }
+    if (FULL || l < tl.count) store_at<T, V>(out, tl.at(l, D * E) + cw * E, o);
+  }
+}
+
+// One block: one tile of 128 positions of 32 * V channels of one sample.
+template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
-  typedef vec_io<T, V> io;
   constexpr int W = kCL * V;
-  __shared__ float lds_a[2][kTG][W];
-  __shared__ float lds_b[2][kTG][W];
-  const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
-  const int64_t cbs = (p.D + W - 1) / W;
-  int64_t bid = blockIdx.x;
-  const int64_t cb = bid % cbs;
-  bid /= cbs;
-  const int64_t b = bid % p.n;
-  const int seg = static_cast<int>(bid / p.n);
-  const int64_t c = cb * W + cl * V;
-  const bool on = c < p.D;
-  const int64_t len = live_length(p.lengths, b, p.T);
-  const int64_t s0 = seg * p.seg;
-  const int64_t s1 = s0 + p.seg < p.T ? s0 + p.seg : p.T;
-  const T* gx = static_cast<const T*>(p.gates) + b * p.sn + c;
-  T* out = static_cast<T*>(p.out) + b * p.T * p.D + c;
-  const int64_t nD = p.n * p.D, row = b * p.D + c;
-
-  float sp[V], h_in[V], prod[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) sp[j] = h_in[j] = 0.f, prod[j] = 1.f;
-  if (on) {
-    load_decay<V>(p.decay, p.decay_bf16, c, sp);
-#pragma unroll
-    for (int j = 0; j < V; ++j) sp[j] = softplus_f(sp[j]);
-    if (!SUMMARY) {
-      if (p.state) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) h_in[j] = p.state[row + j];
-      }
-      for (int k = 0; k < seg; ++k) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          h_in[j] = fmaf(p.sum_a[k * nD + row + j], h_in[j], p.sum_b[k * nD + row + j]);
-      }
-    }
-  }
-
-  int buf = 0;
-  for (int64_t tile = s0; tile < s1; tile += kFwdTile, buf ^= 1) {
-    const int64_t s = tile + tg * kFwdK;
-    typename io::raw rx[kFwdK], rr[kFwdK], ri[kFwdK];
-    bool live[kFwdK];
-#pragma unroll
-    for (int k = 0; k < kFwdK; ++k) {
-      const int64_t pos = p.reverse ? p.T - 1 - (s + k) : s + k;
-      live[k] = on && s + k < s1 && pos < len;
-      rx[k] = rr[k] = ri[k] = typename io::raw();
-      if (live[k]) {
-        const T* q = gx + pos * p.st;
-        rx[k] = io::load(q);
-        rr[k] = io::load(q + p.D);
-        ri[k] = io::load(q + 2 * p.D);
-      }
-    }
-    float a[kFwdK][V], u[kFwdK][V], A[V], B[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kFwdK; ++k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float q;
-        const float L = live[k] ? -sp[j] * sigmoid_f(io::get(rr[k], j)) : 0.f;
-        decay_of(L, a[k][j], q);
-        const float m2 = q * (1.0f + a[k][j]);
-        u[k][j] = m2 * inv_scale(m2) * sigmoid_f(io::get(ri[k], j)) * io::get(rx[k], j);
-        A[j] *= a[k][j];
-        B[j] = fmaf(a[k][j], B[j], u[k][j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) lds_a[buf][tg][cl * V + j] = A[j], lds_b[buf][tg][cl * V + j] = B[j];
-    __syncthreads();  // the other buffer's readers are past it once every thread is here
-    float h[V];
-#pragma unroll
-    for (int g = 0; g < kTG; ++g) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (g == tg) h[j] = h_in[j];
-        const float ga = lds_a[buf][g][cl * V + j];
-        h_in[j] = fmaf(ga, h_in[j], lds_b[buf][g][cl * V + j]);
-        if (SUMMARY) prod[j] *= ga;
-      }
-    }
-    if (!SUMMARY) {
-      if (p.kept && on && s < s1 && s % kChunk == 0) {
-        float* kp = p.kept + (b * ((p.T + kChunk - 1) / kChunk) + s / kChunk) * p.D + c;
-#pragma unroll
-        for (int j = 0; j < V; ++j) kp[j] = h[j];
-      }
-#pragma unroll
-      for (int k = 0; k < kFwdK; ++k) {
-        float o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          h[j] = fmaf(a[k][j], h[j], u[k][j]);
-          o[j] = live[k] ? h[j] : 0.f;
-        }
-        if (on && s + k < s1) io::store(out + (p.reverse ? p.T - 1 - (s + k) : s + k) * p.D, o);
-      }
-    }
-  }
-  if (on && tg == 0) {
-    if (SUMMARY) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) p.sum_a[seg * nD + row + j] = prod[j], p.sum_b[seg * nD + row + j] = h_in[j];
-    } else if (seg == p.S - 1) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) p.last[row + j] = h_in[j];
-    }
-  }
+  __shared__ float lds_a[kTG][W];
+  __shared__ float lds_b[kTG][W];
+  __shared__ float lds_m[2 * kRun * W];
+  __shared__ float lds_s[W];
+  __shared__ int lds_t;
+  const int64_t cbs = (p.D + W - 1) / W, r = blockIdx.x % p.ch.rows, b = r / cbs, cb = r - b * cbs;
+  const int t = __builtin_amdgcn_readfirstlane(draw_tile(p.ch, r, &lds_t));
+  const Tile tl = tile_of<kFwdTile>(p.T, live_length(p.lengths, b, p.T), static_cast<int64_t>(t) * kFwdTile, p.reverse);
+  if (tl.hi - tl.lo == kFwdTile && (cb + 1) * W <= p.D) fwd_tile<T, V, true>(p, t, r, b, cb, tl, lds_a, lds_b, lds_m, lds_s);
+  else fwd_tile<T, V, false>(p, t, r, b, cb, tl, lds_a, lds_b, lds_m, lds_s);
 }
 
-// The reverse recurrence's (A, B) of a segment: needs the decay gates and the output gradients only.
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_bwd_summary_kernel(ScanBwdArgs p) {
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
+                                         float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float (*lds_g)[kCL * V],
+                                         float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
-  constexpr int W = kCL * V;
-  __shared__ float lds_a[2][kTG][W];
-  __shared__ float lds_b[2][kTG][W];
+  constexpr int W = kCL * V, K = kBwdK, E = sizeof(T);
   const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
-  const int64_t cbs = (p.D + W - 1) / W;
-  int64_t bid = blockIdx.x;
-  const int64_t cb = bid % cbs;
-  bid /= cbs;
-  const int64_t b = bid % p.n;
-  const int seg = static_cast<int>(bid / p.n);
-  const int64_t c = cb * W + cl * V;
-  const bool on = c < p.D;
-  const int64_t len = live_length(p.lengths, b, p.T);
-  const int64_t s0 = seg * p.seg;
-  const int64_t s1 = s0 + p.seg < p.T ? s0 + p.seg : p.T;
-  const T* gr = static_cast<const T*>(p.gates) + b * p.sn + p.D + c;
-  const T* dy = static_cast<const T*>(p.dy) + b * p.T * p.D + c;
-  float sp[V], R[V], prod[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) sp[j] = R[j] = 0.f, prod[j] = 1.f;
-  if (on) {
-    load_decay<V>(p.decay, p.decay_bf16, c, sp);
-#pragma unroll
-    for (int j = 0; j < V; ++j) sp[j] = softplus_f(sp[j]);
-  }
-  int buf = 0;
-  const int64_t tiles = s1 > s0 ? (s1 - s0 + kFwdTile - 1) / kFwdTile : 0;
-  for (int64_t i = tiles - 1; i >= 0; --i, buf ^= 1) {
-    const int64_t s = s0 + i * kFwdTile + tg * kFwdK;
-    typename io::raw rr[kFwdK], rd[kFwdK];
-    bool live[kFwdK];
-#pragma unroll
-    for (int k = 0; k < kFwdK; ++k) {
-      const int64_t pos = p.reverse ? p.T - 1 - (s + k) : s + k;
-      live[k] = on && s + k < s1 && pos < len;
-      rr[k] = rd[k] = typename io::raw();
-      if (live[k]) {
-        rr[k] = io::load(gr + pos * p.st);
-        rd[k] = io::load(dy + pos * p.D);
-      }
-    }
-    float A[V], B[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = 0.f;
-#pragma unroll
-    for (int k = kFwdK - 1; k >= 0; --k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float a, q;
-        decay_of(live[k] ? -sp[j] * sigmoid_f(io::get(rr[k], j)) : 0.f, a, q);
-        A[j] *= a;
-        B[j] = a * (io::get(rd[k], j) + B[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) lds_a[buf][tg][cl * V + j] = A[j], lds_b[buf][tg][cl * V + j] = B[j];
-    __syncthreads();
-#pragma unroll
-    for (int g = kTG - 1; g >= 0; --g) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float ga = lds_a[buf][g][cl * V + j];
-        R[j] = fmaf(ga, R[j], lds_b[buf][g][cl * V + j]);
-        prod[j] *= ga;
-      }
-    }
-  }
-  if (on && tg == 0) {
-    const int64_t nD = p.n * p.D, row = b * p.D + c;
-#pragma unroll
-    for (int j = 0; j < V; ++j) p.sum_a[seg * nD + row + j] = prod[j], p.sum_b[seg * nD + row + j] = R[j];
-  }
-}
+  const int cw = cl * V, c = static_cast<int>(cb) * W + cw;
+  const bool on = FULL || c < p.D;
+  const int D = static_cast<int>(p.D), st = static_cast<int>(p.st);
+  const int tile = p.ch.tiles - 1 - t;
+  const T* gx = static_cast<const T*>(p.gates) + b * p.sn + tl.low * p.st + cb * W;
+  const T *gr = gx + D, *gi = gr + D;
+  const T* dy = static_cast<const T*>(p.dy) + (b * p.T + tl.low) * p.D + cb * W;
 
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanBwdArgs p) {
-  typedef vec_io<T, V> io;
-  constexpr int W = kCL * V, K = kBwdK;
-  __shared__ float lds_a[2][kTG][W];
-  __shared__ float lds_b[2][kTG][W];
-  __shared__ float lds_g[2][kTG][W];
-  const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
-  const int64_t cbs = (p.D + W - 1) / W;
-  int64_t bid = blockIdx.x;
-  const int64_t cb = bid % cbs;
-  bid /= cbs;
-  const int64_t b = bid % p.n;
-  const int seg = static_cast<int>(bid / p.n);
-  const int64_t c = cb * W + cl * V;
-  const bool on = c < p.D;
-  const int64_t len = live_length(p.lengths, b, p.T);
-  const int64_t s0 = seg * p.seg;
-  const int64_t s1 = s0 + p.seg < p.T ? s0 + p.seg : p.T;
-  const int64_t chunks = (p.T + kChunk - 1) / kChunk;
-  const T* gx = static_cast<const T*>(p.gates) + b * p.sn + c;
-  const T* dy = static_cast<const T*>(p.dy) + b * p.T * p.D + c;
-  T* dg = static_cast<T*>(p.dgates) + b * p.T * 3 * p.D + c;
+  typename io::raw rx[K], rr[K], ri[K], rd[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int l = tg * K + k;
+    if (!FULL) rx[k] = rr[k] = ri[k] = rd[k] = typename io::raw();
+    if (FULL || (on && l >= tl.lo && l < tl.hi)) {
+      const uint32_t q = tl.at(l, st * E) + cw * E;
+      rx[k] = load_at<T, V>(gx, q);
+      rr[k] = load_at<T, V>(gr, q);
+      ri[k] = load_at<T, V>(gi, q);
+      rd[k] = load_at<T, V>(dy, tl.at(l, D * E) + cw * E);
+    }
+  }
   const int64_t nD = p.n * p.D, row = b * p.D + c;
-
-  float sp[V], ratio[V], R[V], acc[V];
+  float sp[V], ratio[V], h[V], g[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) sp[j] = ratio[j] = R[j] = acc[j] = 0.f;
+  for (int j = 0; j < V; ++j) sp[j] = ratio[j] = h[j] = g[j] = 0.f;
   if (on) {
     load_decay<V>(p.decay, p.decay_bf16, c, sp);
+    typename vec_io<float, V>::raw kh = typename vec_io<float, V>::raw();
+    if (p.T > 0) kh = vec_io<float, V>::load(p.kept + (b * p.ch.tiles + tile) * p.D + c);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       ratio[j] = decay_ratio(sp[j]);
       sp[j] = softplus_f(sp[j]);
-      if (p.dlast) R[j] = p.dlast[row + j];
-    }
-    for (int k = p.S - 1; k > seg; --k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) R[j] = fmaf(p.sum_a[k * nD + row + j], R[j], p.sum_b[k * nD + row + j]);
+      h[j] = vec_io<float, V>::get(kh, j);
+      if (p.dlast && t < kRun) g[j] = p.dlast[row + j];
     }
   }
-
-  int buf = 0;
-  const int64_t tiles = s1 > s0 ? (s1 - s0 + kBwdTile - 1) / kBwdTile : 0;
-  for (int64_t i = tiles - 1; i >= 0; --i, buf ^= 1) {
-    const int64_t tile = s0 + i * kBwdTile;
-    const int64_t s = tile + tg * K;
-    typename io::raw rx[K], rr[K], ri[K], rd[K];
-    bool live[K];
+  // what the second half needs of each element; the rest is a product or two away
+  float a[K][V], m[K][V], im[K][V], sg[K][V], rho[K][V];
+  float A[V], B[V], G[V];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t pos = p.reverse ? p.T - 1 - (s + k) : s + k;
-      live[k] = on && s + k < s1 && pos < len;
-      rx[k] = rr[k] = ri[k] = rd[k] = typename io::raw();
-      if (live[k]) {
-        const T* q = gx + pos * p.st;
-        rx[k] = io::load(q);
-        rr[k] = io::load(q + p.D);
-        ri[k] = io::load(q + 2 * p.D);
-        rd[k] = io::load(dy + pos * p.D);
-      }
-    }
-    float h[V];
+  for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = G[j] = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = on ? p.kept[(b * chunks + tile / kChunk) * p.D + c + j] : 0.f;
-
-    float a[K][V], ms[K][V], sx[K][V], s1m[K][V], r1m[K][V], Lv[K][V], ak[K][V];
-    float A[V], B[V], G[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = G[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float q;
-        const float rho = sigmoid_f(io::get(rr[k], j));
-        const float L = live[k] ? -sp[j] * rho : 0.f;
-        decay_of(L, a[k][j], q);
-        const float m2 = q * (1.0f + a[k][j]), im = inv_scale(m2), m = m2 * im;
-        const float sg = sigmoid_f(io::get(ri[k], j)), x = io::get(rx[k], j);
-        Lv[k][j] = L * a[k][j];
-        ak[k][j] = a[k][j] * a[k][j] * (-L * im);
-        sx[k][j] = sg * x;
-        ms[k][j] = m * sg;
-        s1m[k][j] = x * (1.0f - sg);
-        r1m[k][j] = 1.0f - rho;
-        A[j] *= a[k][j];
-        B[j] = fmaf(a[k][j], B[j], m * sx[k][j]);
-      }
-    }
-#pragma unroll
-    for (int k = K - 1; k >= 0; --k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) G[j] = a[k][j] * (io::get(rd[k], j) + G[j]);
-    }
+  for (int k = 0; k < K; ++k) {
+    const bool live = FULL || (tg * K + k >= tl.lo && tg * K + k < tl.hi);
+    float L[V], q[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      lds_a[buf][tg][cl * V + j] = A[j];
-      lds_b[buf][tg][cl * V + j] = B[j];
-      lds_g[buf][tg][cl * V + j] = G[j];
+      rho[k][j] = sigmoid_f(io::get(rr[k], j));
+      L[j] = live ? -sp[j] * rho[k][j] : 0.f;
     }
-    __syncthreads();
-    float g[V];
+    decay_of<V>(L, a[k], q);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      for (int t = 0; t < tg; ++t) h[j] = fmaf(lds_a[buf][t][cl * V + j], h[j], lds_b[buf][t][cl * V + j]);
-    }
-#pragma unroll
-    for (int t = kTG - 1; t >= 0; --t) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (t == tg) g[j] = R[j];
-        R[j] = fmaf(lds_a[buf][t][cl * V + j], R[j], lds_g[buf][t][cl * V + j]);
-      }
-    }
-    float hp[K][V];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        hp[k][j] = h[j];
-        h[j] = fmaf(a[k][j], h[j], ms[k][j] * io::get(rx[k], j));
-      }
-    }
-#pragma unroll
-    for (int k = K - 1; k >= 0; --k) {
-      float ox[V], orr[V], oi[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float gt = io::get(rd[k], j) + g[j];
-        g[j] = a[k][j] * gt;
-        const float w = gt * fmaf(Lv[k][j], hp[k][j], sx[k][j] * ak[k][j]);
-        const float dx = gt * ms[k][j];
-        acc[j] += w;
-        ox[j] = live[k] ? dx : 0.f;
-        orr[j] = live[k] ? w * r1m[k][j] : 0.f;
-        oi[j] = live[k] ? dx * s1m[k][j] : 0.f;
-      }
-      if (on && s + k < s1) {
-        T* q = dg + (p.reverse ? p.T - 1 - (s + k) : s + k) * 3 * p.D;
-        io::store(q, ox);
-        io::store(q + p.D, orr);
-        io::store(q + 2 * p.D, oi);
-      }
+      const float m2 = fmaf(q[j], a[k][j], q[j]);
+      im[k][j] = inv_scale(m2);
+      m[k][j] = m2 * im[k][j];
+      sg[k][j] = sigmoid_f(io::get(ri[k], j));
+      A[j] *= a[k][j];
+      B[j] = fmaf(a[k][j], B[j], m[k][j] * sg[k][j] * io::get(rx[k], j));
     }
   }
-  // sum_t w of the segment over the time groups, in order
+#pragma unroll
+  for (int k = K - 1; k >= 0; --k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) G[j] = a[k][j] * (io::get(rd[k], j) + G[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) lds_a[tg][cw + j] = A[j], lds_b[tg][cw + j] = B[j], lds_g[tg][cw + j] = G[j];
+  __syncthreads();
+  float TA[V], TG[V], PA[V], PG[V];
+  fold_groups<V, true>(lds_a, lds_g, cl, tg, PA, PG, TA, TG);
+  through_chain<V>(p.ch, r, t, cl, tg, TA, TG, g, lds_m, lds_s);
+  if (on && tg == 0 && p.dstate && tile == 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.dstate[row + j] = fmaf(TA[j], g[j], TG[j]);
+  }
+#pragma unroll
+  for (int o = 0; o < kTG; ++o) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float n = fmaf(lds_a[o][cw + j], h[j], lds_b[o][cw + j]);
+      h[j] = o < tg ? n : h[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) g[j] = fmaf(PA[j], g[j], PG[j]);
+  // The products below are formed again, not kept from the first half: the empty asm makes the
+  // compiler take the factors as new values, which keeps a thread's registers down.
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) asm volatile("" : "+v"(m[k][j]), "+v"(sg[k][j]), "+v"(rho[k][j]), "+v"(im[k][j]));
+  }
+  float hp[K][V], acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      hp[k][j] = h[j];
+      h[j] = fmaf(a[k][j], h[j], m[k][j] * sg[k][j] * io::get(rx[k], j));
+    }
+  }
+  T* dg = static_cast<T*>(p.dgates) + (b * p.T + tl.low) * 3 * p.D + cb * W;
+  T *dr = dg + D, *di = dr + D;
+#pragma unroll
+  for (int k = K - 1; k >= 0; --k) {
+    const int l = tg * K + k;
+    const bool live = FULL || (l >= tl.lo && l < tl.hi);
+    float ox[V], orr[V], oi[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float gt = io::get(rd[k], j) + g[j], x = io::get(rx[k], j);
+      g[j] = a[k][j] * gt;
+      // w = g (L a h_{t-1} + s x a^2 kappa), kappa = -L / m
+      const float L = -sp[j] * rho[k][j];
+      const float w = g[j] * fmaf(L, hp[k][j], -(L * im[k][j]) * (sg[k][j] * x * a[k][j]));
+      const float dx = gt * m[k][j] * sg[k][j];
+      acc[j] += live ? w : 0.f;
+      ox[j] = live ? dx : 0.f;
+      orr[j] = live ? fmaf(-w, rho[k][j], w) : 0.f;
+      oi[j] = live ? dx * fmaf(-x, sg[k][j], x) : 0.f;
+    }
+    if (FULL || (on && l < tl.count)) {
+      const uint32_t q = tl.at(l, 3 * D * E) + cw * E;
+      store_at<T, V>(dg, q, ox);
+      store_at<T, V>(dr, q, orr);
+      store_at<T, V>(di, q, oi);
+    }
+  }
+  if (!p.dlam) return;
+  // sum_t w of the tile over the time groups, in order
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < V; ++j) lds_a[0][tg][cl * V + j] = acc[j];
+  for (int j = 0; j < V; ++j) lds_g[tg][cw + j] = acc[j];
   __syncthreads();
   if (on && tg == 0) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float t = 0.f;
-      for (int g = 0; g < kTG; ++g) t += lds_a[0][g][cl * V + j];
-      if (p.dlam) p.dlam[seg * nD + row + j] = t * ratio[j];
-      if (p.dstate && seg == 0) p.dstate[row + j] = R[j];
+      float sum = 0.f;
+#pragma unroll
+      for (int o = 0; o < kTG; ++o) sum += lds_g[o][cw + j];
+      p.dlam[tile * nD + row + j] = sum * ratio[j];
     }
   }
 }
 
-__global__ __launch_bounds__(kThreads) void scan_dlam_kernel(const float* __restrict__ part, int S, int64_t nD,
-                                                             float* __restrict__ out) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= nD) return;
+// One block: one tile of 64 positions, from the row's last to its first.
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanBwdArgs p) {
+  constexpr int W = kCL * V;
+  __shared__ float lds_a[kTG][W];
+  __shared__ float lds_b[kTG][W];
+  __shared__ float lds_g[kTG][W];
+  __shared__ float lds_m[2 * kRun * W];
+  __shared__ float lds_s[W];
+  __shared__ int lds_t;
+  const int64_t cbs = (p.D + W - 1) / W, r = blockIdx.x % p.ch.rows, b = r / cbs, cb = r - b * cbs;
+  const int t = __builtin_amdgcn_readfirstlane(draw_tile(p.ch, r, &lds_t));  // 0 is the last tile of the scan
+  const Tile tl = tile_of<kBwdTile>(p.T, live_length(p.lengths, b, p.T),
+                                    static_cast<int64_t>(p.ch.tiles - 1 - t) * kBwdTile, p.reverse);
+  if (tl.hi - tl.lo == kBwdTile && (cb + 1) * W <= p.D)
+    bwd_tile<T, V, true>(p, t, r, b, cb, tl, lds_a, lds_b, lds_g, lds_m, lds_s);
+  else
+    bwd_tile<T, V, false>(p, t, r, b, cb, tl, lds_a, lds_b, lds_g, lds_m, lds_s);
+}
+
+// out[i] = sum over the tiles of part[tile][i]: 64 sums a block, 16 waves each on every 16th tile.
+__global__ __launch_bounds__(1024) void scan_dlam_kernel(const float* __restrict__ part, int tiles, int64_t nD,
+                                                         float* __restrict__ out) {
+  __shared__ float lds[16][DPK_WAVE];
+  const int lane = threadIdx.x % DPK_WAVE, wave = threadIdx.x / DPK_WAVE;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * DPK_WAVE + lane;
   float t = 0.f;
-  for (int s = 0; s < S; ++s) t += part[s * nD + i];
-  out[i] = t;
+  if (i < nD) {
+#pragma unroll 4
+    for (int k = wave; k < tiles; k += 16) t += part[k * nD + i];
+  }
+  lds[wave][lane] = t;
+  __syncthreads();
+  if (wave == 0 && i < nD) {
+    t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t += lds[w][lane];
+    out[i] = t;
+  }
 }
 
 template <typename T, int V>
@@ -497,33 +592,48 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(const T* __restrict
   const typename vec_io<float, V>::raw rh = vec_io<float, V>::load(state + b * D + c);
   float lam[V], h[V];
   load_decay<V>(decay, decay_bf16, c, lam);
+  float L[V], a[V], q[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) L[j] = -softplus_f(lam[j]) * sigmoid_f(io::get(rr, j));
+  decay_of<V>(L, a, q);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    float a, q;
-    decay_of(-softplus_f(lam[j]) * sigmoid_f(io::get(rr, j)), a, q);
-    const float m2 = q * (1.0f + a);
-    h[j] = fmaf(a, vec_io<float, V>::get(rh, j), m2 * inv_scale(m2) * sigmoid_f(io::get(ri, j)) * io::get(rx, j));
+    const float m = __builtin_amdgcn_sqrtf(fmaf(q[j], a[j], q[j]));
+    h[j] = fmaf(a[j], vec_io<float, V>::get(rh, j), m * sigmoid_f(io::get(ri, j)) * io::get(rx, j));
   }
   vec_io<float, V>::store(state + b * D + c, h);
   io::store(out + b * D + c, h);
 }
 
-// Segments of T for n samples of D channels: enough blocks to fill the GPU, whole tiles each.
-void segments_of(int64_t n, int64_t T, int64_t D, int V, int* S, int64_t* seg) {
-  const int64_t rows = n * dpk_cdiv(D, kCL * V), tiles = dpk_cdiv(T, kFwdTile);
-  int64_t want = rows > 0 ? dpk_cdiv(kWantBlocks, rows) : 1;
-  if (rows * 2 > kWantBlocks) want = 1;
-  if (want > kMaxSegments) want = kMaxSegments;
-  if (want > tiles) want = tiles;
-  if (want < 1) want = 1;
-  const int64_t per = dpk_cdiv(tiles > 0 ? tiles : 1, want);
-  *S = static_cast<int>(dpk_cdiv(tiles > 0 ? tiles : 1, per));
-  *seg = per * kFwdTile;
+int tiles_of(int64_t T, int tile) { return T > tile ? static_cast<int>(dpk_cdiv(T, tile)) : 1; }
+
+// The chain's part of the workspace for rows of 16 * V channels: tickets, maps, states.
+size_t chain_bytes(int64_t n, int64_t D, int V, int tiles) {
+  if (tiles == 1) return 0;
+  const size_t rows = static_cast<size_t>(n * dpk_cdiv(D, kCL * V));
+  return dpk_align_up(rows * 4, 256) + rows * kCL * V * 8 * (tiles + dpk_cdiv(tiles, kRun));
+}
+// Sets up and clears the chain of a launch; returns the first byte behind it.
+char* chain_of(Chain* ch, int64_t n, int64_t D, int V, int tiles, void* ws, hipStream_t s) {
+  ch->rows = n * dpk_cdiv(D, kCL * V);
+  ch->tiles = tiles;
+  ch->runs = static_cast<int>(dpk_cdiv(tiles, kRun));
+  if (tiles == 1) return static_cast<char*>(ws);
+  const int64_t W = kCL * V, words = ch->rows * W * (tiles + ch->runs);
+  char* at = static_cast<char*>(ws);
+  ch->tickets = reinterpret_cast<uint32_t*>(at);
+  at += dpk_align_up(static_cast<size_t>(ch->rows) * 4, 256);
+  ch->maps = reinterpret_cast<uint64_t*>(at);
+  ch->states = ch->maps + ch->rows * tiles * W;
+  const int64_t blocks = dpk_cdiv(words, kThreads * 4);
+  hipLaunchKernelGGL(chain_clear_kernel, dim3(static_cast<unsigned>(blocks < 2048 ? blocks : 2048)), dim3(kThreads), 0, s,
+                     ch->tickets, ch->rows, ch->maps, words);
+  return at + words * 8;
 }
 
-int vec_of(int64_t D, int dtype, int64_t sn, int64_t st, int64_t n, int64_t T, std::initializer_list<const void*> elems,
+int vec_of(int most, int64_t D, int dtype, int64_t sn, int64_t st, int64_t n, int64_t T, std::initializer_list<const void*> elems,
            std::initializer_list<const void*> floats) {
-  for (int V = 4; V > 1; V /= 2) {
+  for (int V = most; V > 1; V /= 2) {
     bool ok = D % V == 0 && (n == 1 || sn % V == 0) && (T == 1 || st % V == 0);
     for (const void* e : elems) ok = ok && dpk_aligned(e, dpk_elsize(dtype) * V);
     for (const void* f : floats) ok = ok && dpk_aligned(f, 4 * V);
@@ -544,21 +654,24 @@ int check_common(const char* fn, const void* gates, int dtype, const void* decay
   DPK_REQUIRE(dpk_aligned(gates, dpk_elsize(dtype)) && dpk_aligned(decay, dpk_elsize(decay_dtype)), DPK_E_ALIGN,
               "%s: gates or decay not aligned to its element size", fn);
   DPK_REQUIRE(sn >= 0 && st >= 0, DPK_E_ARG, "%s: negative stride", fn);
-  DPK_REQUIRE(n * dpk_cdiv(D, kCL) * kMaxSegments <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: n * D too large", fn);
+  DPK_REQUIRE(3 * D <= kMaxStride && (T <= 1 || st <= kMaxStride), DPK_E_SHAPE,
+              "%s: a position's features span more than %lld elements", fn, (long long)kMaxStride);
+  DPK_REQUIRE(T < (1LL << 36) && n < (1LL << 31) && D < (1LL << 31) && dpk_cdiv(T + 1, kBwdTile) * dpk_cdiv(D, kCL) * n <= DPK_MAX_GRID_X,
+              DPK_E_SHAPE, "%s: n * T * D too large", fn);
   return DPK_OK;
 }
 
 }  // namespace
 
 extern "C" size_t dpk_gated_scan_workspace_bytes(int64_t n, int64_t T, int64_t D) {
-  if (n <= 0 || T <= 0 || D <= 0) return 0;
-  int S;
-  int64_t seg, most = 1;
-  for (int V = 1; V <= 4; V *= 2) {  // whichever width the pointers allow
-    segments_of(n, T, D, V, &S, &seg);
-    if (S > most) most = S;
+  if (n <= 0 || T <= kBwdTile || D <= 0) return 0;
+  const int tiles = tiles_of(T, kBwdTile);  // the backward pass cuts finer
+  size_t most = 0;
+  for (int V = 1; V <= 2; V *= 2) {  // whichever width the pointers allow
+    const size_t need = chain_bytes(n, D, V, tiles);
+    if (need > most) most = need;
   }
-  return most > 1 ? dpk_align_up(static_cast<size_t>(3) * most * n * D * 4, 256) : 0;
+  return dpk_align_up(most + static_cast<size_t>(tiles) * n * D * 4, 256);
 }
 
 extern "C" int dpk_gated_scan(const void* gates, int dtype, const void* decay, int decay_dtype, const float* state,
@@ -573,32 +686,22 @@ extern "C" int dpk_gated_scan(const void* gates, int dtype, const void* decay, i
   DPK_REQUIRE(dpk_aligned(out, dpk_elsize(dtype)) && dpk_aligned(last, 4) && dpk_aligned(state, 4) && dpk_aligned(kept, 4) &&
                   dpk_aligned(lengths, 8),
               DPK_E_ALIGN, "%s: a tensor is not aligned to its element size", fn);
-  const int V = vec_of(D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, out}, {last, state, kept});
-  ScanArgs p = {gates, decay, state, lengths, out, last, kept, nullptr, nullptr, n, T, D, gates_stride_n, gates_stride_t,
-                decay_dtype == DPK_BF16, reverse, 1, 0};
-  segments_of(n, T, D, V, &p.S, &p.seg);
-  if (p.S > 1) {
-    DPK_REQUIRE(ws && ws_bytes >= dpk_gated_scan_workspace_bytes(n, T, D), DPK_E_WORKSPACE, "%s: workspace too small (%zu)",
-                fn, ws_bytes);
-    DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
-    p.sum_a = static_cast<float*>(ws);
-    p.sum_b = p.sum_a + static_cast<int64_t>(p.S) * n * D;
-  }
+  const int V = vec_of(2, D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, out}, {last, state, kept});
+  const int tiles = tiles_of(T, kFwdTile);
+  const size_t need = chain_bytes(n, D, V, tiles);
+  DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
+  DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t rows = n * dpk_cdiv(D, kCL * V);
-#define DPK_SCAN_FWD(TT, VV)                                                                                              \
-  do {                                                                                                                    \
-    if (p.S > 1)                                                                                                          \
-      hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, true>), dim3((unsigned)(rows * (p.S - 1))), dim3(kThreads), 0, s, p);   \
-    hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, false>), dim3((unsigned)(rows * p.S)), dim3(kThreads), 0, s, p);          \
-  } while (0)
+  ScanArgs p = {gates, decay, state, lengths, out, last, kept, n, T, D, gates_stride_n, gates_stride_t,
+                decay_dtype == DPK_BF16, reverse, {}};
+  chain_of(&p.ch, n, D, V, tiles, ws, s);
+  const dim3 grid(static_cast<unsigned>(p.ch.rows * tiles));
+#define DPK_SCAN_FWD(TT, VV) hipLaunchKernelGGL((scan_fwd_kernel<TT, VV>), grid, dim3(kThreads), 0, s, p)
   if (dtype == DPK_BF16) {
-    if (V == 4) DPK_SCAN_FWD(bf16_t, 4);
-    else if (V == 2) DPK_SCAN_FWD(bf16_t, 2);
+    if (V == 2) DPK_SCAN_FWD(bf16_t, 2);
     else DPK_SCAN_FWD(bf16_t, 1);
   } else {
-    if (V == 4) DPK_SCAN_FWD(float, 4);
-    else if (V == 2) DPK_SCAN_FWD(float, 2);
+    if (V == 2) DPK_SCAN_FWD(float, 2);
     else DPK_SCAN_FWD(float, 1);
   }
 #undef DPK_SCAN_FWD
@@ -620,40 +723,30 @@ extern "C" int dpk_gated_scan_backward(const void* gates, int dtype, const void*
                   dpk_aligned(grad_last, 4) && dpk_aligned(grad_decay, 4) && dpk_aligned(grad_state, 4) &&
                   dpk_aligned(lengths, 8),
               DPK_E_ALIGN, "%s: a tensor is not aligned to its element size", fn);
-  const int V = vec_of(D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, grad_out, grad_gates},
+  const int V = vec_of(2, D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, grad_out, grad_gates},
                        {kept, grad_last, grad_decay, grad_state});
-  ScanBwdArgs p = {gates, decay, kept, lengths, grad_out, grad_last, grad_gates, grad_state, grad_decay, nullptr, nullptr,
-                   n, T, D, gates_stride_n, gates_stride_t, decay_dtype == DPK_BF16, reverse, 1, 0};
-  segments_of(n, T, D, V, &p.S, &p.seg);
-  if (p.S > 1) {
-    DPK_REQUIRE(ws && ws_bytes >= dpk_gated_scan_workspace_bytes(n, T, D), DPK_E_WORKSPACE, "%s: workspace too small (%zu)",
-                fn, ws_bytes);
-    DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
-    p.sum_a = static_cast<float*>(ws);
-    p.sum_b = p.sum_a + static_cast<int64_t>(p.S) * n * D;
-    if (grad_decay) p.dlam = p.sum_b + static_cast<int64_t>(p.S) * n * D;
-  }
+  const int tiles = tiles_of(T, kBwdTile);
+  const size_t need = chain_bytes(n, D, V, tiles) + (tiles > 1 && grad_decay ? static_cast<size_t>(tiles) * n * D * 4 : 0);
+  DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
+  DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t rows = n * dpk_cdiv(D, kCL * V);
-#define DPK_SCAN_BWD(TT, VV)                                                                                            \
-  do {                                                                                                                  \
-    if (p.S > 1)                                                                                                        \
-      hipLaunchKernelGGL((scan_bwd_summary_kernel<TT, VV>), dim3((unsigned)(rows * p.S)), dim3(kThreads), 0, s, p);     \
-    hipLaunchKernelGGL((scan_bwd_kernel<TT, VV>), dim3((unsigned)(rows * p.S)), dim3(kThreads), 0, s, p);               \
-  } while (0)
+  ScanBwdArgs p = {gates, decay, kept, lengths, grad_out, grad_last, grad_gates, grad_state, grad_decay, n, T, D,
+                   gates_stride_n, gates_stride_t, decay_dtype == DPK_BF16, reverse, {}};
+  char* behind = chain_of(&p.ch, n, D, V, tiles, ws, s);
+  if (tiles > 1 && grad_decay) p.dlam = reinterpret_cast<float*>(behind);
+  const dim3 grid(static_cast<unsigned>(p.ch.rows * tiles));
+#define DPK_SCAN_BWD(TT, VV) hipLaunchKernelGGL((scan_bwd_kernel<TT, VV>), grid, dim3(kThreads), 0, s, p)
   if (dtype == DPK_BF16) {
-    if (V == 4) DPK_SCAN_BWD(bf16_t, 4);
-    else if (V == 2) DPK_SCAN_BWD(bf16_t, 2);
+    if (V == 2) DPK_SCAN_BWD(bf16_t, 2);
     else DPK_SCAN_BWD(bf16_t, 1);
   } else {
-    if (V == 4) DPK_SCAN_BWD(float, 4);
-    else if (V == 2) DPK_SCAN_BWD(float, 2);
+    if (V == 2) DPK_SCAN_BWD(float, 2);
     else DPK_SCAN_BWD(float, 1);
   }
 #undef DPK_SCAN_BWD
-  if (p.S > 1 && grad_decay)
-    hipLaunchKernelGGL(scan_dlam_kernel, dim3((unsigned)dpk_cdiv(n * D, kThreads)), dim3(kThreads), 0, s, p.dlam, p.S, n * D,
-                       grad_decay);
+  if (tiles > 1 && grad_decay)
+    hipLaunchKernelGGL(scan_dlam_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * D, DPK_WAVE))), dim3(1024), 0, s, p.dlam, tiles,
+                       n * D, grad_decay);
   DPK_LAUNCH_CHECK(fn);
   return DPK_OK;
 }
@@ -666,7 +759,7 @@ extern "C" int dpk_gated_scan_step(const void* gates, int dtype, const void* dec
   DPK_REQUIRE(state && out, DPK_E_ARG, "%s: state or out is NULL", fn);
   DPK_REQUIRE(dpk_aligned(out, dpk_elsize(dtype)) && dpk_aligned(state, 4), DPK_E_ALIGN,
               "%s: a tensor is not aligned to its element size", fn);
-  const int V = vec_of(D, dtype, gates_stride_n, 0, n, 1, {gates, out}, {state});
+  const int V = vec_of(4, D, dtype, gates_stride_n, 0, n, 1, {gates, out}, {state});
   const unsigned grid = static_cast<unsigned>(dpk_cdiv(n * (D / V), kThreads));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int db = decay_dtype == DPK_BF16;
