@@ -44,12 +44,6 @@ __device__ __forceinline__ float softplus_f(float v) {
   const float l = d > 0.f ? __builtin_amdgcn_logf(u) * 0.69314718055994531f * (e * __builtin_amdgcn_rcpf(d)) : e;
   return fmaxf(v, 0.f) + l;
 }
-// sigma(v) / softplus(v); 1 in the limit v -> -inf, where both are exp(v)
-__device__ __forceinline__ float decay_ratio(float v) {
-  const float sp = softplus_f(v);
-  return sp > 0.f ? sigmoid_f(v) / sp : 1.0f;
-}
-
 // For the decay gates of one position: L = -softplus(lam) sigma(r), a = exp(L) and q = 1 - a, each
 // to its own relative accuracy: q = -L P(L) while L > -0.7, P the degree-5 polynomial nearest to
 // (exp(L) - 1) / L there (1e-8 of it off; found by Remez exchange), q = 1 - a beyond. A layer starts out
@@ -128,33 +122,41 @@ __device__ __forceinline__ void await(const uint64_t* w, float* a, float* b) {
   }
 }
 
-__global__ __launch_bounds__(kThreads) void chain_clear_kernel(uint32_t* tickets, int64_t rows, uint64_t* words, int64_t count) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < count; i += step) words[i] = ~0ull;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < rows; i += step) tickets[i] = 0;
+// pairs: 16-byte pairs of words; the tickets lie in front of them.
+__global__ __launch_bounds__(kThreads) void chain_clear_kernel(uint32_t* tickets, int64_t rows, uint4* pairs, int64_t count) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads, first = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  for (int64_t i = first; i < count; i += step) pairs[i] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
+  for (int64_t i = first; i < rows; i += step) tickets[i] = 0;
 }
 
-// This block's tile number in its row, in the order of the chain.
-__device__ __forceinline__ int draw_tile(const Chain& ch, int64_t row, int* lds) {
-  if (ch.tiles == 1) return 0;
-  if (threadIdx.x == 0) *lds = static_cast<int>(__hip_atomic_fetch_add(ch.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+// This block's tile number in its row, in the order of the chain: drawn first, read once the work that
+// does not depend on it is under way.
+__device__ __forceinline__ void draw_tile(const Chain& ch, int64_t row, int* lds) {
+  if (threadIdx.x == 0)
+    *lds = ch.tiles == 1 ? 0 : static_cast<int>(__hip_atomic_fetch_add(ch.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ int drawn_tile(const int* lds) {
   __syncthreads();
-  return *lds;
+  return __builtin_amdgcn_readfirstlane(*lds);
 }
 
-// The state that enters tile `t` of the row whose own map is (TA, TB) and whose first state is `in`
-// (which receives it). All threads call it; lds: [2][kRun][W] and [W] floats nobody else uses.
+// Tile t's own map (TA, TB), for the tiles behind it in its run.
 template <int V>
-__device__ __forceinline__ void through_chain(const Chain& ch, int64_t row, int t, int cl, int tg, const float (&TA)[V],
-                                              const float (&TB)[V], float (&in)[V], float* lds_m, float* lds_s) {
-  constexpr int W = kCL * V;
-  const int run = t / kRun, k = t - run * kRun;
-  const bool more = t + 1 < ch.tiles;
-  if (more && k + 1 < kRun && tg == 0) {
-    uint64_t* w = ch.maps + (row * ch.tiles + t) * W + cl * V;
+__device__ __forceinline__ void publish_map(const Chain& ch, int64_t row, int t, int cl, int tg, const float (&TA)[V],
+                                            const float (&TB)[V]) {
+  if (tg == 0 && t + 1 < ch.tiles && t % kRun + 1 < kRun) {
+    uint64_t* w = ch.maps + (row * ch.tiles + t) * (kCL * V) + cl * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) publish(w + j, TA[j], TB[j]);
   }
+}
+// The state that enters tile t, in `in`, which holds the row's first state. All threads call it;
+// lds_m: [2][kRun][W], lds_s: [W], used by nothing else.
+template <int V>
+__device__ __forceinline__ void state_before(const Chain& ch, int64_t row, int t, int cl, int tg, const float (&TA)[V],
+                                             const float (&TB)[V], float (&in)[V], float* lds_m, float* lds_s) {
+  constexpr int W = kCL * V;
+  const int run = t / kRun, k = t - run * kRun;
   if (t > 0) {
     float x[V], y[V];
     for (int g = tg; g < k; g += kTG) {
@@ -177,7 +179,7 @@ __device__ __forceinline__ void through_chain(const Chain& ch, int64_t row, int 
       for (int j = 0; j < V; ++j) in[j] = fmaf(lds_m[g * W + cl * V + j], in[j], lds_m[(kRun + g) * W + cl * V + j]);
     }
   }
-  if (more && k + 1 == kRun && tg == 0) {
+  if (tg == 0 && t + 1 < ch.tiles && k + 1 == kRun) {
     uint64_t* w = ch.states + (row * ch.runs + run + 1) * W + cl * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) publish(w + j, 0.f, fmaf(TA[j], in[j], TB[j]));
@@ -219,6 +221,17 @@ __device__ __forceinline__ void load_decay(const void* decay, int is_bf16, int64
     lam[j] = is_bf16 ? bf16_to_f32(static_cast<const bf16_t*>(decay)[c + j]) : static_cast<const float*>(decay)[c + j];
 }
 
+// softplus of the decays of V channels from c on; 0 behind the last channel
+template <int V>
+__device__ __forceinline__ void softplus_of(const void* decay, int is_bf16, int64_t D, int64_t c, float (&sp)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) sp[j] = 0.f;
+  if (c >= D) return;
+  load_decay<V>(decay, is_bf16, c, sp);
+#pragma unroll
+  for (int j = 0; j < V; ++j) sp[j] = softplus_f(sp[j]);
+}
+
 __device__ __forceinline__ int64_t live_length(const int64_t* lengths, int64_t b, int64_t T) {
   if (!lengths) return T;
   const int64_t l = lengths[b];
@@ -234,6 +247,17 @@ struct Tile {
   bool reverse;
   __device__ __forceinline__ int at(int l, int stride) const { return (reverse ? count - 1 - l : l) * stride; }
 };
+// Where position k of a thread's K lies in a FULL tile: the same 32-bit byte offset for all k, and
+// for each k a step of the block's base, which is scalar arithmetic.
+template <int K>
+__device__ __forceinline__ uint32_t first_of(const Tile& t, int tg, int stride_bytes) {
+  return (t.reverse ? t.count - K - tg * K : tg * K) * stride_bytes;
+}
+template <int K>
+__device__ __forceinline__ int64_t step_of(const Tile& t, int k, int stride) {
+  return static_cast<int64_t>(t.reverse ? K - 1 - k : k) * stride;
+}
+
 template <typename T, int V>
 __device__ __forceinline__ typename vec_io<T, V>::raw load_at(const T* base, uint32_t bytes) {
   return vec_io<T, V>::load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + bytes));
@@ -264,7 +288,7 @@ __device__ __forceinline__ void fold_groups(const float (*la)[kCL * V], const fl
                                             float (&PA)[V], float (&PB)[V], float (&TA)[V], float (&TB)[V]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) TA[j] = PA[j] = 1.f, TB[j] = PB[j] = 0.f;
-#pragma unroll
+#pragma unroll 2  // (all eight unrolled, the LDS reads in flight alone would cost a wave of occupancy)
   for (int i = 0; i < kTG; ++i) {
     const int g = BACK ? kTG - 1 - i : i;
 #pragma unroll
@@ -280,7 +304,7 @@ __device__ __forceinline__ void fold_groups(const float (*la)[kCL * V], const fl
 // FULL: every position and channel of the tile is live.
 template <typename T, int V, bool FULL>
 __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
-                                         float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float* lds_m, float* lds_s) {
+                                         const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
   constexpr int W = kCL * V, K = kFwdK, E = sizeof(T);
   const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
@@ -296,25 +320,17 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
     const int l = tg * K + k;
     if (!FULL) rx[k] = rr[k] = ri[k] = typename io::raw();
     if (FULL || (on && l >= tl.lo && l < tl.hi)) {
-      const uint32_t q = tl.at(l, st * E) + cw * E;
-      rx[k] = load_at<T, V>(gx, q);
-      rr[k] = load_at<T, V>(gr, q);
-      ri[k] = load_at<T, V>(gi, q);
+      const uint32_t q = (FULL ? first_of<K>(tl, tg, st * E) : tl.at(l, st * E)) + cw * E;
+      const int64_t at = FULL ? step_of<K>(tl, k, st) : 0;
+      rx[k] = load_at<T, V>(gx + at, q);
+      rr[k] = load_at<T, V>(gr + at, q);
+      ri[k] = load_at<T, V>(gi + at, q);
     }
   }
   const int64_t row = b * p.D + c;
-  float sp[V], h[V];
+  float h[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) sp[j] = h[j] = 0.f;
-  if (on) {
-    load_decay<V>(p.decay, p.decay_bf16, c, sp);
-#pragma unroll
-    for (int j = 0; j < V; ++j) sp[j] = softplus_f(sp[j]);
-    if (p.state && t < kRun) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) h[j] = p.state[row + j];
-    }
-  }
+  for (int j = 0; j < V; ++j) h[j] = on && p.state && t < kRun ? p.state[row + j] : 0.f;
   float a[K][V], u[K][V], A[V], B[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = 0.f;
@@ -338,7 +354,8 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
   __syncthreads();
   float TA[V], TB[V], PA[V], PB[V];
   fold_groups<V, false>(lds_a, lds_b, cl, tg, PA, PB, TA, TB);
-  through_chain<V>(p.ch, r, t, cl, tg, TA, TB, h, lds_m, lds_s);
+  publish_map<V>(p.ch, r, t, cl, tg, TA, TB);
+  state_before<V>(p.ch, r, t, cl, tg, TA, TB, h, lds_m, lds_s);
   if (on && tg == 0 && t + 1 == p.ch.tiles) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.last[row + j] = fmaf(TA[j], h[j], TB[j]);
@@ -361,13 +378,14 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
       h[j] = fmaf(a[k][j], h[j], u[k][j]);
       o[j] = live ? h[j] : 0.f;
     }
-    if (FULL || l < tl.count) store_at<T, V>(out, tl.at(l, D * E) + cw * E, o);
+    if (FULL) store_at<T, V>(out + step_of<K>(tl, k, D), first_of<K>(tl, tg, D * E) + cw * E, o);
+    else if (l < tl.count) store_at<T, V>(out, tl.at(l, D * E) + cw * E, o);
   }
 }
 
 // One block: one tile of 128 positions of 32 * V channels of one sample.
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_kernel(ScanArgs p) {
   constexpr int W = kCL * V;
   __shared__ float lds_a[kTG][W];
   __shared__ float lds_b[kTG][W];
@@ -375,15 +393,18 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
   __shared__ float lds_s[W];
   __shared__ int lds_t;
   const int64_t cbs = (p.D + W - 1) / W, r = blockIdx.x % p.ch.rows, b = r / cbs, cb = r - b * cbs;
-  const int t = __builtin_amdgcn_readfirstlane(draw_tile(p.ch, r, &lds_t));
+  draw_tile(p.ch, r, &lds_t);
+  float sp[V];
+  softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
+  const int t = drawn_tile(&lds_t);
   const Tile tl = tile_of<kFwdTile>(p.T, live_length(p.lengths, b, p.T), static_cast<int64_t>(t) * kFwdTile, p.reverse);
-  if (tl.hi - tl.lo == kFwdTile && (cb + 1) * W <= p.D) fwd_tile<T, V, true>(p, t, r, b, cb, tl, lds_a, lds_b, lds_m, lds_s);
-  else fwd_tile<T, V, false>(p, t, r, b, cb, tl, lds_a, lds_b, lds_m, lds_s);
+  if (tl.hi - tl.lo == kFwdTile && (cb + 1) * W <= p.D) fwd_tile<T, V, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
+  else fwd_tile<T, V, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
 }
 
 template <typename T, int V, bool FULL>
 __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
-                                         float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float (*lds_g)[kCL * V],
+                                         const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float (*lds_g)[kCL * V],
                                          float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
   constexpr int W = kCL * V, K = kBwdK, E = sizeof(T);
@@ -402,31 +423,26 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
     const int l = tg * K + k;
     if (!FULL) rx[k] = rr[k] = ri[k] = rd[k] = typename io::raw();
     if (FULL || (on && l >= tl.lo && l < tl.hi)) {
-      const uint32_t q = tl.at(l, st * E) + cw * E;
-      rx[k] = load_at<T, V>(gx, q);
-      rr[k] = load_at<T, V>(gr, q);
-      ri[k] = load_at<T, V>(gi, q);
-      rd[k] = load_at<T, V>(dy, tl.at(l, D * E) + cw * E);
+      const uint32_t q = (FULL ? first_of<K>(tl, tg, st * E) : tl.at(l, st * E)) + cw * E;
+      const uint32_t q1 = (FULL ? first_of<K>(tl, tg, D * E) : tl.at(l, D * E)) + cw * E;
+      const int64_t at = FULL ? step_of<K>(tl, k, st) : 0, at1 = FULL ? step_of<K>(tl, k, D) : 0;
+      rx[k] = load_at<T, V>(gx + at, q);
+      rr[k] = load_at<T, V>(gr + at, q);
+      ri[k] = load_at<T, V>(gi + at, q);
+      rd[k] = load_at<T, V>(dy + at1, q1);
     }
   }
   const int64_t nD = p.n * p.D, row = b * p.D + c;
-  float sp[V], ratio[V], h[V], g[V];
+  float h[V], g[V];
+  typename vec_io<float, V>::raw kh = typename vec_io<float, V>::raw();
+  if (on && p.T > 0) kh = vec_io<float, V>::load(p.kept + (b * p.ch.tiles + tile) * p.D + c);
 #pragma unroll
-  for (int j = 0; j < V; ++j) sp[j] = ratio[j] = h[j] = g[j] = 0.f;
-  if (on) {
-    load_decay<V>(p.decay, p.decay_bf16, c, sp);
-    typename vec_io<float, V>::raw kh = typename vec_io<float, V>::raw();
-    if (p.T > 0) kh = vec_io<float, V>::load(p.kept + (b * p.ch.tiles + tile) * p.D + c);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      ratio[j] = decay_ratio(sp[j]);
-      sp[j] = softplus_f(sp[j]);
-      h[j] = vec_io<float, V>::get(kh, j);
-      if (p.dlast && t < kRun) g[j] = p.dlast[row + j];
-    }
+  for (int j = 0; j < V; ++j) {
+    h[j] = vec_io<float, V>::get(kh, j);
+    g[j] = on && p.dlast && t < kRun ? p.dlast[row + j] : 0.f;
   }
   // what the second half needs of each element; the rest is a product or two away
-  float a[K][V], m[K][V], im[K][V], sg[K][V], rho[K][V];
+  float a[K][V], ms[K][V], is[K][V], sg[K][V], rho[K][V];  // ms = m s, is = s / m
   float A[V], B[V], G[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = G[j] = 0.f;
@@ -443,11 +459,11 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float m2 = fmaf(q[j], a[k][j], q[j]);
-      im[k][j] = inv_scale(m2);
-      m[k][j] = m2 * im[k][j];
       sg[k][j] = sigmoid_f(io::get(ri[k], j));
+      is[k][j] = inv_scale(m2) * sg[k][j];
+      ms[k][j] = m2 * is[k][j];
       A[j] *= a[k][j];
-      B[j] = fmaf(a[k][j], B[j], m[k][j] * sg[k][j] * io::get(rx[k], j));
+      B[j] = fmaf(a[k][j], B[j], ms[k][j] * io::get(rx[k], j));
     }
   }
 #pragma unroll
@@ -460,12 +476,9 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
   __syncthreads();
   float TA[V], TG[V], PA[V], PG[V];
   fold_groups<V, true>(lds_a, lds_g, cl, tg, PA, PG, TA, TG);
-  through_chain<V>(p.ch, r, t, cl, tg, TA, TG, g, lds_m, lds_s);
-  if (on && tg == 0 && p.dstate && tile == 0) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) p.dstate[row + j] = fmaf(TA[j], g[j], TG[j]);
-  }
-#pragma unroll
+  publish_map<V>(p.ch, r, t, cl, tg, TA, TG);
+  // the states inside the tile, while the words of the chain are on their way
+#pragma unroll 2
   for (int o = 0; o < kTG; ++o) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -473,14 +486,12 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
       h[j] = o < tg ? n : h[j];
     }
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) g[j] = fmaf(PA[j], g[j], PG[j]);
   // The products below are formed again, not kept from the first half: the empty asm makes the
   // compiler take the factors as new values, which keeps a thread's registers down.
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) asm volatile("" : "+v"(m[k][j]), "+v"(sg[k][j]), "+v"(rho[k][j]), "+v"(im[k][j]));
+    for (int j = 0; j < V; ++j) asm volatile("" : "+v"(ms[k][j]), "+v"(sg[k][j]), "+v"(rho[k][j]), "+v"(is[k][j]));
   }
   float hp[K][V], acc[V];
 #pragma unroll
@@ -490,9 +501,16 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       hp[k][j] = h[j];
-      h[j] = fmaf(a[k][j], h[j], m[k][j] * sg[k][j] * io::get(rx[k], j));
+      h[j] = fmaf(a[k][j], h[j], ms[k][j] * io::get(rx[k], j));
     }
   }
+  state_before<V>(p.ch, r, t, cl, tg, TA, TG, g, lds_m, lds_s);
+  if (on && tg == 0 && p.dstate && tile == 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.dstate[row + j] = fmaf(TA[j], g[j], TG[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) g[j] = fmaf(PA[j], g[j], PG[j]);
   T* dg = static_cast<T*>(p.dgates) + (b * p.T + tl.low) * 3 * p.D + cb * W;
   T *dr = dg + D, *di = dr + D;
 #pragma unroll
@@ -504,20 +522,22 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
     for (int j = 0; j < V; ++j) {
       const float gt = io::get(rd[k], j) + g[j], x = io::get(rx[k], j);
       g[j] = a[k][j] * gt;
-      // w = g (L a h_{t-1} + s x a^2 kappa), kappa = -L / m
-      const float L = -sp[j] * rho[k][j];
-      const float w = g[j] * fmaf(L, hp[k][j], -(L * im[k][j]) * (sg[k][j] * x * a[k][j]));
-      const float dx = gt * m[k][j] * sg[k][j];
-      acc[j] += live ? w : 0.f;
+      // w = g (L a h_{t-1} + s x a^2 kappa) with kappa = -L / m and L = -softplus rho:
+      // w / -softplus = a g rho (h_{t-1} - a x s / m)
+      const float v = g[j] * rho[k][j] * fmaf(-is[k][j], x * a[k][j], hp[k][j]);
+      const float w = -sp[j] * v;
+      const float dx = gt * ms[k][j];
+      acc[j] += live ? v : 0.f;
       ox[j] = live ? dx : 0.f;
       orr[j] = live ? fmaf(-w, rho[k][j], w) : 0.f;
       oi[j] = live ? dx * fmaf(-x, sg[k][j], x) : 0.f;
     }
     if (FULL || (on && l < tl.count)) {
-      const uint32_t q = tl.at(l, 3 * D * E) + cw * E;
-      store_at<T, V>(dg, q, ox);
-      store_at<T, V>(dr, q, orr);
-      store_at<T, V>(di, q, oi);
+      const uint32_t q = (FULL ? first_of<K>(tl, tg, 3 * D * E) : tl.at(l, 3 * D * E)) + cw * E;
+      const int64_t at = FULL ? step_of<K>(tl, k, 3 * D) : 0;
+      store_at<T, V>(dg + at, q, ox);
+      store_at<T, V>(dr + at, q, orr);
+      store_at<T, V>(di + at, q, oi);
     }
   }
   if (!p.dlam) return;
@@ -532,14 +552,15 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
       float sum = 0.f;
 #pragma unroll
       for (int o = 0; o < kTG; ++o) sum += lds_g[o][cw + j];
-      p.dlam[tile * nD + row + j] = sum * ratio[j];
+      // sigma(lam) / softplus(lam) times the -softplus(lam) that v lacks of w; lam is short of one here
+      p.dlam[tile * nD + row + j] = -sum * -expm1f(-sp[j]);
     }
   }
 }
 
 // One block: one tile of 64 positions, from the row's last to its first.
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanBwdArgs p) {
+__global__ __launch_bounds__(kThreads, 3) void scan_bwd_kernel(ScanBwdArgs p) {
   constexpr int W = kCL * V;
   __shared__ float lds_a[kTG][W];
   __shared__ float lds_b[kTG][W];
@@ -548,13 +569,16 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanBwdArgs p) {
   __shared__ float lds_s[W];
   __shared__ int lds_t;
   const int64_t cbs = (p.D + W - 1) / W, r = blockIdx.x % p.ch.rows, b = r / cbs, cb = r - b * cbs;
-  const int t = __builtin_amdgcn_readfirstlane(draw_tile(p.ch, r, &lds_t));  // 0 is the last tile of the scan
+  draw_tile(p.ch, r, &lds_t);
+  float sp[V];
+  softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
+  const int t = drawn_tile(&lds_t);  // 0 is the last tile of the scan
   const Tile tl = tile_of<kBwdTile>(p.T, live_length(p.lengths, b, p.T),
                                     static_cast<int64_t>(p.ch.tiles - 1 - t) * kBwdTile, p.reverse);
   if (tl.hi - tl.lo == kBwdTile && (cb + 1) * W <= p.D)
-    bwd_tile<T, V, true>(p, t, r, b, cb, tl, lds_a, lds_b, lds_g, lds_m, lds_s);
+    bwd_tile<T, V, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_g, lds_m, lds_s);
   else
-    bwd_tile<T, V, false>(p, t, r, b, cb, tl, lds_a, lds_b, lds_g, lds_m, lds_s);
+    bwd_tile<T, V, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_g, lds_m, lds_s);
 }
 
 // out[i] = sum over the tiles of part[tile][i]: 64 sums a block, 16 waves each on every 16th tile.
@@ -625,9 +649,9 @@ char* chain_of(Chain* ch, int64_t n, int64_t D, int V, int tiles, void* ws, hipS
   at += dpk_align_up(static_cast<size_t>(ch->rows) * 4, 256);
   ch->maps = reinterpret_cast<uint64_t*>(at);
   ch->states = ch->maps + ch->rows * tiles * W;
-  const int64_t blocks = dpk_cdiv(words, kThreads * 4);
+  const int64_t blocks = dpk_cdiv(words, kThreads * 4);  // two 16-byte stores a thread
   hipLaunchKernelGGL(chain_clear_kernel, dim3(static_cast<unsigned>(blocks < 2048 ? blocks : 2048)), dim3(kThreads), 0, s,
-                     ch->tickets, ch->rows, ch->maps, words);
+                     ch->tickets, ch->rows, reinterpret_cast<uint4*>(ch->maps), words / 2);
   return at + words * 8;
 }
 
