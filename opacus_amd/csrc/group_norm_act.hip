@@ -78,6 +78,7 @@ struct NormArgs {
   int64_t n, S;
   int C, G, Cg;
   int cl;               // vectors of a row that a block covers
+  int lg;               // lanes of a group (statistics per position)
   int cblocks;          // blocks along a row
   int J;                // row chunks of a sample
   int64_t chunk;        // rows of one
@@ -405,7 +406,195 @@ __global__ __launch_bounds__(kThreads) void sample_dx_kernel(NormArgs p) {
   }
 }
 
-// ---- statistics per position, any group size: one wave per (row, group) -----------------------
+// ---- statistics per position: the groups of a row side by side in the lanes of a wave ------------
+//
+// A group takes `lg` lanes (the least power of two that holds its vectors, NI vectors a lane where 64
+// lanes are not enough), a wave 64 / lg groups of one row and the same groups of the next rows, so a
+// row's sums are a few lane exchanges, and the columns a lane holds never change: weight and
+// bias stay in registers, and so do the per-sample sums along the rows. Nothing is read twice.
+
+// v[i] = sum of v[i] over the lg lanes of the group, in all of them.
+template <int R>
+__device__ __forceinline__ void lane_sum(float (&v)[R], int lg) {
+#define DPK_DPP_STEP(at, ctrl)                                                                                       \
+  if (lg > at) {                                                                                                     \
+    _Pragma("unroll") for (int i = 0; i < R; ++i) v[i] += __int_as_float(                                            \
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v[i]), ctrl, 0xf, 0xf, true));                                 \
+  }
+  DPK_DPP_STEP(1, 0xb1)   // quad_perm [1,0,3,2]
+  DPK_DPP_STEP(2, 0x4e)   // quad_perm [2,3,0,1]
+  DPK_DPP_STEP(4, 0x141)  // row_half_mirror
+  DPK_DPP_STEP(8, 0x140)  // row_mirror
+#undef DPK_DPP_STEP
+  if (lg > 16) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] += __shfl_xor(v[i], 16, DPK_WAVE);
+  }
+  if (lg > 32) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] += __shfl_xor(v[i], 32, DPK_WAVE);
+  }
+}
+
+template <typename T, int V, int NI, int R, bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
+  typedef vec_io<T, V> io;
+  constexpr int N = NI * V, kWaves = kThreads / DPK_WAVE;
+  __shared__ float lds[BACKWARD ? 2 : 1][BACKWARD ? kWaves : 1][BACKWARD ? DPK_WAVE * N : 1];
+  const int lane = threadIdx.x % DPK_WAVE, wave = threadIdx.x / DPK_WAVE;
+  const int cb = static_cast<int>(blockIdx.x % p.cblocks);
+  const int64_t rest = blockIdx.x / p.cblocks;
+  // forward: row chunks of the whole tensor; backward: of one sample
+  const int64_t b = BACKWARD ? rest / p.J : 0, j = BACKWARD ? rest - b * p.J : rest;
+  const int64_t rows = BACKWARD ? p.S : p.n * p.S;
+  const int64_t r0 = j * p.chunk, r1 = r0 + p.chunk < rows ? r0 + p.chunk : rows;
+  const int g = cb * (DPK_WAVE / p.lg) + lane / p.lg, at = lane % p.lg;
+  const bool mine = g < p.G;
+  bool on[NI];
+  int c[NI];
+  float w[N], shift[N];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int in = (i * p.lg + at) * V;
+    on[i] = mine && in < p.Cg;
+    c[i] = on[i] ? g * p.Cg + in : 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      w[i * V + k] = on[i] ? param_at(p.w, p.param_bf16, c[i] + k, 1.f) : 0.f;
+      shift[i * V + k] = on[i] ? param_at(p.b, p.param_bf16, c[i] + k, 0.f) : 0.f;
+    }
+  }
+  const float inv = 1.0f / static_cast<float>(p.Cg);
+  const T* x = static_cast<const T*>(p.x) + b * p.S * p.C;
+  const T* dy = static_cast<const T*>(p.dy) + b * p.S * p.C;
+  T* y = static_cast<T*>(p.y) + b * p.S * p.C;
+  float A[N], B[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) A[k] = B[k] = 0.f;
+
+  for (int64_t r = r0 + wave * R; r < r1; r += kWaves * R) {
+    typename io::raw rx[R][NI], rd[R][NI];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        rx[q][i] = rd[q][i] = typename io::raw();
+        if (on[i] && r + q < r1) {
+          rx[q][i] = io::load(x + (r + q) * p.C + c[i]);
+          if (BACKWARD) rd[q][i] = io::load(dy + (r + q) * p.C + c[i]);
+        }
+      }
+    }
+    float mean[R], rstd[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) mean[q] += io::get(rx[q][i], k);
+      }
+    }
+    lane_sum(mean, p.lg);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] *= inv;
+      rstd[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = io::get(rx[q][i], k) - mean[q];
+          rstd[q] = on[i] ? fmaf(d, d, rstd[q]) : rstd[q];
+        }
+      }
+    }
+    lane_sum(rstd, p.lg);
+#pragma unroll
+    for (int q = 0; q < R; ++q) rstd[q] = 1.0f / sqrtf(fmaf(rstd[q], inv, p.eps));
+    if (!BACKWARD) {
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          float z[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            z[k] = fmaf((io::get(rx[q][i], k) - mean[q]) * rstd[q], w[i * V + k], shift[i * V + k]);
+          activate(z, p.act);
+          if (on[i] && r + q < r1) io::store(y + (r + q) * p.C + c[i], z);
+        }
+      }
+    } else {
+      float s1[R], s2[R], xh[R][N], d[R][N];
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        s1[q] = s2[q] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          float z[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            xh[q][i * V + k] = (io::get(rx[q][i], k) - mean[q]) * rstd[q];
+            z[k] = fmaf(xh[q][i * V + k], w[i * V + k], shift[i * V + k]);
+          }
+          slope(z, p.act);
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            // a row behind the last one has dy = 0, but its slope may not be a number times zero
+            const float dz = r + q < r1 ? io::get(rd[q][i], k) * z[k] : 0.f;
+            A[i * V + k] += dz;
+            B[i * V + k] = r + q < r1 ? fmaf(dz, xh[q][i * V + k], B[i * V + k]) : B[i * V + k];
+            d[q][i * V + k] = dz * w[i * V + k];
+            s1[q] += d[q][i * V + k];
+            s2[q] = on[i] ? fmaf(d[q][i * V + k], xh[q][i * V + k], s2[q]) : s2[q];
+          }
+        }
+      }
+      lane_sum(s1, p.lg);
+      lane_sum(s2, p.lg);
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        s1[q] *= inv;
+        s2[q] *= inv;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          float o[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) o[k] = rstd[q] * (d[q][i * V + k] - s1[q] - xh[q][i * V + k] * s2[q]);
+          if (on[i] && r + q < r1) io::store(y + (r + q) * p.C + c[i], o);
+        }
+      }
+    }
+  }
+  if (!BACKWARD) return;
+  if (!p.gw && !p.gb) return;
+#pragma unroll
+  for (int k = 0; k < N; ++k) lds[0][wave][k * DPK_WAVE + lane] = A[k], lds[BACKWARD][wave][k * DPK_WAVE + lane] = B[k];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float t = 0.f, u = 0.f;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) {
+        t += lds[0][BACKWARD ? v : 0][(i * V + k) * DPK_WAVE + lane];
+        u += lds[BACKWARD][BACKWARD ? v : 0][(i * V + k) * DPK_WAVE + lane];
+      }
+      if (!on[i]) continue;
+      if (p.J > 1) {
+        p.part[(b * p.J + j) * p.C + c[i] + k] = make_float2(t, u);
+      } else {
+        if (p.gb) p.gb[b * p.C + c[i] + k] = t;
+        if (p.gw) p.gw[b * p.C + c[i] + k] = u;
+      }
+    }
+  }
+}
+
+// ---- statistics per position, groups that no wave holds: one wave per (row, group) ---------------
 
 template <typename T, bool BACKWARD>
 __global__ __launch_bounds__(kThreads) void position_kernel(NormArgs p) {
@@ -502,6 +691,29 @@ int width_of(const NormArgs& p, int dtype) {
   return 1;
 }
 
+// Statistics per position: the widest loads for which a group's vectors fit into a wave, up to 4 a
+// lane. False if none do.
+bool plan_rows(NormArgs* p, int dtype, bool backward, int* V, int* NI) {
+  for (*V = dtype == DPK_BF16 ? 8 : 4;; *V /= 2) {
+    const size_t al = dpk_elsize(dtype) * *V;
+    if (p->Cg % *V == 0 && dpk_aligned(p->x, al) && dpk_aligned(p->dy, al) && dpk_aligned(p->y, al)) break;
+  }
+  const int vecs = p->Cg / *V;
+  for (p->lg = 1; p->lg < vecs && p->lg < DPK_WAVE;) p->lg *= 2;
+  for (*NI = 1; *NI * p->lg < vecs;) *NI *= 2;
+  if (*NI > 4) return false;
+  p->cblocks = static_cast<int>(dpk_cdiv(p->G, DPK_WAVE / p->lg));
+  const int64_t rows = backward ? p->S : p->n * p->S, samples = backward ? p->n : 1;
+  // enough blocks to fill the GPU; backward, no chunk below 64 rows (the partial sums of one cost 8 bytes a channel)
+  int64_t J = dpk_cdiv(kWantBlocks, samples * p->cblocks);
+  const int64_t most = dpk_cdiv(rows, backward ? 64 : 4);
+  if (J > most) J = most;
+  if (J < 1) J = 1;
+  p->chunk = dpk_cdiv(rows, J);
+  p->J = static_cast<int>(dpk_cdiv(rows, p->chunk));
+  return true;
+}
+
 size_t part_bytes(int64_t n, int64_t S, int64_t C) {
   size_t most = 0;
   for (int V = 1; V <= 8; V *= 2) {  // whichever width the pointers allow
@@ -512,6 +724,10 @@ size_t part_bytes(int64_t n, int64_t S, int64_t C) {
     const size_t need = static_cast<size_t>(n) * p.J * C * sizeof(float2);
     if (need > most) most = need;
   }
+  // statistics per position cut a sample into no more chunks than 64-row ones, nor than it takes to fill the GPU
+  int64_t J = dpk_cdiv(S, 64);
+  if (J > dpk_cdiv(kWantBlocks, n)) J = dpk_cdiv(kWantBlocks, n);
+  if (static_cast<size_t>(n) * J * C * sizeof(float2) > most) most = static_cast<size_t>(n) * J * C * sizeof(float2);
   return dpk_align_up(most, 256);
 }
 size_t group_bytes(int64_t n, int64_t S, int64_t G, int per_position) {
@@ -545,6 +761,14 @@ int check_common(const char* fn, const NormArgs& p, int dtype, int param_dtype, 
   DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
   DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
   return DPK_OK;
+}
+
+template <typename T, int V, bool BACKWARD>
+void launch_rows(const NormArgs& p, int NI, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((BACKWARD ? p.n : 1) * p.J * p.cblocks)), block(kThreads);
+  if (NI == 1) hipLaunchKernelGGL((position_rows_kernel<T, V, 1, BACKWARD ? 2 : 4, BACKWARD>), grid, block, 0, s, p);
+  else if (NI == 2) hipLaunchKernelGGL((position_rows_kernel<T, V, 2, BACKWARD ? 1 : 2, BACKWARD>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((position_rows_kernel<T, V, 4, 1, BACKWARD>), grid, block, 0, s, p);
 }
 
 // Calls body(T{}, integral_constant<V>) for the tensor's type and width.
@@ -582,12 +806,16 @@ extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, 
   DPK_REQUIRE(stats || per_position, DPK_E_ARG, "%s: stats is NULL", fn);
   p.C = static_cast<int>(C), p.G = static_cast<int>(groups), p.Cg = p.C / p.G;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (per_position) {
+  int V, NI;
+  if (per_position && plan_rows(&p, dtype, false, &V, &NI)) {
+    DPK_REQUIRE(static_cast<int64_t>(p.J) * p.cblocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+    by_width(dtype, V, [&](auto t, auto v) { launch_rows<decltype(t), decltype(v)::value, false>(p, NI, s); });
+  } else if (per_position) {
     const unsigned grid = static_cast<unsigned>(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE));
     if (dtype == DPK_BF16) hipLaunchKernelGGL((position_kernel<bf16_t, false>), dim3(grid), dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL((position_kernel<float, false>), dim3(grid), dim3(kThreads), 0, s, p);
   } else {
-    const int V = width_of(p, dtype);
+    V = width_of(p, dtype);
     plan(&p, V);
     p.part = static_cast<float2*>(ws);
     const int64_t blocks = n * p.cblocks * p.J;
@@ -623,12 +851,21 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
   DPK_REQUIRE(stats || per_position, DPK_E_ARG, "%s: stats is NULL", fn);
   p.C = static_cast<int>(C), p.G = static_cast<int>(groups), p.Cg = p.C / p.G;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int V = width_of(p, dtype);
+  p.part = static_cast<float2*>(ws);
+  int V, NI;
+  if (per_position && plan_rows(&p, dtype, true, &V, &NI)) {
+    DPK_REQUIRE(n * p.J * p.cblocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+    by_width(dtype, V, [&](auto t, auto v) { launch_rows<decltype(t), decltype(v)::value, true>(p, NI, s); });
+    if (p.J > 1 && (p.gw || p.gb))
+      hipLaunchKernelGGL(chunk_merge_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * C, kThreads))), dim3(kThreads), 0, s, p);
+    DPK_LAUNCH_CHECK(fn);
+    return DPK_OK;
+  }
+  V = width_of(p, dtype);
   plan(&p, V);
   const int64_t blocks = n * p.cblocks * p.J;
   DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
   const dim3 grid(static_cast<unsigned>(blocks));
-  p.part = static_cast<float2*>(ws);
   float2* groups_ws = reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(n, S, C));
   if (per_position) {
     p.stats = groups_ws;
