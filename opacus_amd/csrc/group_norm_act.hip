@@ -21,10 +21,26 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 8;           // rows a thread has in flight in the streaming kernels
+constexpr int kRows = 8;           // rows a thread has in flight in the statistics kernel
+constexpr int kApplyRows = 4;      // and where it also computes
 constexpr int64_t kWantBlocks = 2048;
 
 constexpr int kRelu = DPK_ACT_RELU, kSilu = DPK_ACT_SILU, kGelu = DPK_ACT_GELU;
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and E = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun:
+// erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2) with t = 1 / (1 + p x), off by at most 1.5e-7. Its
+// exponential is the one act' needs, and for z < 0 no 1 - erf cancels.
+__device__ __forceinline__ float normal_cdf(float z, float& E) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+  E = __builtin_amdgcn_exp2f(x * x * -kLog2e);
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  q *= 0.5f * t * E;
+  return z < 0.f ? q : 1.0f - q;
+}
 
 // z -> act(z) for N values; one uniform branch for all of them.
 template <int N>
@@ -34,7 +50,10 @@ __device__ __forceinline__ void activate(float (&z)[N], int act) {
     for (int i = 0; i < N; ++i) z[i] *= sigmoid_f(z[i]);
   } else if (act == kGelu) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] *= 0.5f * (1.0f + erff(z[i] * 0.70710678118654752f));
+    for (int i = 0; i < N; ++i) {
+      float E;
+      z[i] *= normal_cdf(z[i], E);
+    }
   } else if (act == kRelu) {
 #pragma unroll
     for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : (z[i] != z[i] ? z[i] : 0.f);
@@ -52,8 +71,9 @@ __device__ __forceinline__ void slope(float (&z)[N], int act) {
   } else if (act == kGelu) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float phi = 0.5f * (1.0f + erff(z[i] * 0.70710678118654752f));
-      z[i] = fmaf(z[i] * 0.39894228040143268f, __builtin_amdgcn_exp2f(z[i] * z[i] * (-0.5f * kLog2e)), phi);
+      float E;
+      const float phi = normal_cdf(z[i], E);
+      z[i] = fmaf(z[i] * 0.39894228040143268f, E, phi);
     }
   } else if (act == kRelu) {
 #pragma unroll
@@ -121,7 +141,7 @@ __device__ __forceinline__ Span span_of(const NormArgs& p) {
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void sample_stat_kernel(NormArgs p) {
   typedef vec_io<T, V> io;
-  __shared__ float lds[2][kThreads][V];
+  __shared__ float lds[2][kThreads * V];
   const Span s = span_of<V>(p);
   const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
   float mean[V], m2[V], cnt = 0.f;
@@ -160,26 +180,27 @@ __global__ __launch_bounds__(kThreads) void sample_stat_kernel(NormArgs p) {
       cnt = all;
     }
   }
+  const int W = p.cl * V, lane = threadIdx.x % p.cl;
+  if (s.rg < s.step) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) lds[0][threadIdx.x][j] = mean[j], lds[1][threadIdx.x][j] = m2[j];
+    for (int j = 0; j < V; ++j) lds[0][s.rg * W + lane * V + j] = mean[j], lds[1][s.rg * W + lane * V + j] = m2[j];
+  }
   __syncthreads();
-  if (s.on && s.rg == 0) {
-    // rows of row group g: ceil((rows - g) / step)
-    const int64_t rows = s.r1 - s.r0;
-    const int lane = threadIdx.x;
-    float2* out = p.part + (s.b * p.J + s.j) * p.C + s.c;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float t = 0.f, q = 0.f;
-      for (int g = 0; g < s.step && g < rows; ++g)
-        t += static_cast<float>((rows - g + s.step - 1) / s.step) * lds[0][g * p.cl + lane][j];
-      t /= static_cast<float>(rows);
-      for (int g = 0; g < s.step && g < rows; ++g) {
-        const float d = lds[0][g * p.cl + lane][j] - t;
-        q += fmaf(d * d, static_cast<float>((rows - g + s.step - 1) / s.step), lds[1][g * p.cl + lane][j]);
-      }
-      out[j] = make_float2(t, q);
+  // row group g of the block saw ceil((rows - g) / step) rows
+  const int64_t rows = s.r1 - s.r0;
+  const int groups = rows < s.step ? static_cast<int>(rows) : s.step;
+  const float most = static_cast<float>((rows + s.step - 1) / s.step);
+  const int extra = static_cast<int>(rows - (rows + s.step - 1) / s.step * s.step) + s.step;  // groups below it saw `most`
+  const int c0 = s.c - lane * V;
+  for (int i = threadIdx.x; i < W && c0 + i < p.C; i += kThreads) {
+    float t = 0.f, q = 0.f;
+    for (int g = 0; g < groups; ++g) t = fmaf(g < extra ? most : most - 1.f, lds[0][g * W + i], t);
+    t /= static_cast<float>(rows);
+    for (int g = 0; g < groups; ++g) {
+      const float d = lds[0][g * W + i] - t;
+      q += fmaf(d * d, g < extra ? most : most - 1.f, lds[1][g * W + i]);
     }
+    p.part[(s.b * p.J + s.j) * p.C + c0 + i] = make_float2(t, q);
   }
 }
 
@@ -229,35 +250,35 @@ __global__ __launch_bounds__(kThreads) void sample_apply_kernel(NormArgs p) {
     f[j] = st.y * param_at(p.w, p.param_bf16, s.c + j, 1.f);
     shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
   }
-  for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * kRows) {
-    typename io::raw raw[kRows];
+  for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * kApplyRows) {
+    typename io::raw raw[kApplyRows];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
+    for (int k = 0; k < kApplyRows; ++k) {
       const int64_t at = r + static_cast<int64_t>(k) * s.step;
       raw[k] = typename io::raw();
       if (at < s.r1) raw[k] = io::load(x + at * p.C);
     }
-    float z[kRows * V];
+    float z[kApplyRows * V];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
+    for (int k = 0; k < kApplyRows; ++k) {
 #pragma unroll
       for (int j = 0; j < V; ++j) z[k * V + j] = fmaf(io::get(raw[k], j) - mean[j], f[j], shift[j]);
     }
     activate(z, p.act);
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
+    for (int k = 0; k < kApplyRows; ++k) {
       const int64_t at = r + static_cast<int64_t>(k) * s.step;
       if (at < s.r1) io::store(y + at * p.C, z + k * V);
     }
   }
 }
 
-// (mean, rstd) of one element's statistics: per sample once per thread, per position from the row.
+// part[n,j,c] = (sum dz, sum dz xh) of channel c over the rows of chunk j.
 template <typename T, int V, bool PER_POSITION>
 __global__ __launch_bounds__(kThreads) void channel_sums_kernel(NormArgs p) {
   typedef vec_io<T, V> io;
   constexpr int R = 4;
-  __shared__ float lds[2][kThreads][V];
+  __shared__ float lds[2][kThreads * V];
   const Span s = span_of<V>(p);
   const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
   const T* dy = static_cast<const T*>(p.dy) + (s.b * p.S) * p.C + s.c;
@@ -311,40 +332,54 @@ __global__ __launch_bounds__(kThreads) void channel_sums_kernel(NormArgs p) {
       }
     }
   }
+  const int W = p.cl * V, lane = threadIdx.x % p.cl, c0 = s.c - lane * V;
+  if (s.rg < s.step) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) lds[0][threadIdx.x][j] = A[j], lds[1][threadIdx.x][j] = B[j];
+    for (int j = 0; j < V; ++j) lds[0][s.rg * W + lane * V + j] = A[j], lds[1][s.rg * W + lane * V + j] = B[j];
+  }
   __syncthreads();
-  if (s.on && s.rg == 0) {
-    float2* out = p.part + (s.b * p.J + s.j) * p.C + s.c;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float t = 0.f, q = 0.f;
-      for (int g = 0; g < s.step; ++g) t += lds[0][g * p.cl + threadIdx.x][j], q += lds[1][g * p.cl + threadIdx.x][j];
-      out[j] = make_float2(t, q);
-    }
+  for (int i = threadIdx.x; i < W && c0 + i < p.C; i += kThreads) {
+    float t = 0.f, q = 0.f;
+    for (int g = 0; g < s.step; ++g) t += lds[0][g * W + i], q += lds[1][g * W + i];
+    p.part[(s.b * p.J + s.j) * p.C + c0 + i] = make_float2(t, q);
   }
 }
 
-// gw, gb from the chunks' sums, and S1, S2 of the group. One block per (n, g).
+// gw, gb from the chunks' sums, and S1, S2 of the group. One block per (n, g): up to 256 channels side
+// by side, and as many threads for the chunks of each as that leaves.
 __global__ __launch_bounds__(kThreads) void sample_grad_merge_kernel(NormArgs p) {
   __shared__ float red[kThreads / DPK_WAVE];
+  __shared__ float2 lds[kThreads];
   const int64_t b = blockIdx.x / p.G;
   const int g = static_cast<int>(blockIdx.x % p.G);
+  const int across = p.Cg < kThreads ? p.Cg : kThreads, down = kThreads / across;
+  const int lane = threadIdx.x % across, row = threadIdx.x / across;
   float s1 = 0.f, s2 = 0.f;
-  for (int i = threadIdx.x; i < p.Cg; i += kThreads) {
-    const int c = g * p.Cg + i;
-    const float2* part = p.part + b * p.J * p.C + c;
+  for (int i0 = 0; i0 < p.Cg; i0 += across) {
+    const int c = g * p.Cg + i0 + lane;
+    const bool on = i0 + lane < p.Cg && row < down;
     float A = 0.f, B = 0.f;
-    for (int j = 0; j < p.J; ++j) {
-      const float2 v = part[static_cast<int64_t>(j) * p.C];
-      A += v.x;
-      B += v.y;
+    if (on) {
+      const float2* part = p.part + b * p.J * p.C + c;
+#pragma unroll 4
+      for (int j = row; j < p.J; j += down) {
+        const float2 v = part[static_cast<int64_t>(j) * p.C];
+        A += v.x;
+        B += v.y;
+      }
     }
-    if (p.gb) p.gb[b * p.C + c] = A;
-    if (p.gw) p.gw[b * p.C + c] = B;
-    const float w = param_at(p.w, p.param_bf16, c, 1.f);
-    s1 = fmaf(w, A, s1);
-    s2 = fmaf(w, B, s2);
+    __syncthreads();
+    lds[threadIdx.x] = make_float2(A, B);
+    __syncthreads();
+    if (on && row == 0) {
+      A = B = 0.f;
+      for (int r = 0; r < down; ++r) A += lds[r * across + lane].x, B += lds[r * across + lane].y;
+      if (p.gb) p.gb[b * p.C + c] = A;
+      if (p.gw) p.gw[b * p.C + c] = B;
+      const float w = param_at(p.w, p.param_bf16, c, 1.f);
+      s1 = fmaf(w, A, s1);
+      s2 = fmaf(w, B, s2);
+    }
   }
   s1 = block_sum<kThreads / DPK_WAVE>(s1, red);
   s2 = block_sum<kThreads / DPK_WAVE>(s2, red);
@@ -403,6 +438,168 @@ __global__ __launch_bounds__(kThreads) void sample_dx_kernel(NormArgs p) {
       const int64_t at = r + static_cast<int64_t>(k) * s.step;
       if (at < s.r1) io::store(dx + at * p.C, o);
     }
+  }
+}
+
+// ---- statistics per sample, where a block holds all positions of some whole groups ---------------
+//
+// A block takes gs neighbouring groups (a slab of 128 bytes of each row or more) of one sample, a thread
+// one vector column of every step-th row, all in registers: x (and dy) are read once. Measured at
+// 256 x 32 x 32 x 64 fp32 against partial sums, their merge and a second reading (three launches): see below.
+constexpr int kSlabThreads = 512;
+constexpr int kSlabWidth = 2048;  // channels at most: 56 KB of LDS
+
+// s[i] (i < groups of the slab) = sum over the slab's channels i * Cg ... of w * v, v[V] being this
+// thread's value for its columns: first over the row groups, then over the channels. `chan` keeps the
+// channels' unweighted sums. lds: [step][W].
+template <int V>
+__device__ __forceinline__ void slab_sums(const float (&v)[V], bool on, int rg, int lane, int step, int W, int Cg, float* lds,
+                                          float* chan, float* s, const float* w) {
+  __syncthreads();
+  if (on) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds[rg * W + lane * V + j] = v[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < W; i += kSlabThreads) {
+    float t = 0.f;
+#pragma unroll 4
+    for (int g = 0; g < step; ++g) t += lds[g * W + i];
+    chan[i] = t;
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < W / Cg; g += kSlabThreads) {
+    float t = 0.f;
+    for (int i = g * Cg; i < (g + 1) * Cg; ++i) t = w ? fmaf(w[i], chan[i], t) : t + chan[i];
+    s[g] = t;
+  }
+  __syncthreads();
+}
+
+template <typename T, int V, int R, bool BACKWARD>
+__global__ __launch_bounds__(kSlabThreads) void slab_kernel(NormArgs p) {
+  typedef vec_io<T, V> io;
+  extern __shared__ float shared[];  // [step][W], 2 x [W], 2 x [groups], [W]
+  const int slabs = p.cblocks;
+  const int64_t b = blockIdx.x / slabs;
+  const int slab = static_cast<int>(blockIdx.x - b * slabs);
+  const int g0 = slab * p.lg, gs = p.G - g0 < p.lg ? p.G - g0 : p.lg;  // p.lg: groups of a slab
+  const int W = gs * p.Cg, cl = W / V, step = kSlabThreads / cl;
+  float* lds = shared;
+  float* chan[2] = {lds + kSlabThreads * V, lds + kSlabThreads * V + W};
+  float* grp[2] = {chan[1] + W, chan[1] + W + gs};
+  float* wts = grp[1] + gs;
+  const int lane = threadIdx.x % cl, rg = threadIdx.x / cl;
+  const bool on = rg < step;
+  const int in = lane * V, c = g0 * p.Cg + in;
+  const int S = static_cast<int>(p.S);
+  const T* x = static_cast<const T*>(p.x) + b * p.S * p.C + c;
+  const T* dy = static_cast<const T*>(p.dy) + b * p.S * p.C + c;
+  T* y = static_cast<T*>(p.y) + b * p.S * p.C + c;
+  typename io::raw rx[R], rd[BACKWARD ? R : 1];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int r = rg + k * step;
+    rx[k] = typename io::raw();
+    if (BACKWARD) rd[BACKWARD ? k : 0] = typename io::raw();
+    if (on && r < S) {
+      rx[k] = io::load(x + static_cast<int64_t>(r) * p.C);
+      if (BACKWARD) rd[BACKWARD ? k : 0] = io::load(dy + static_cast<int64_t>(r) * p.C);
+    }
+  }
+  float w[V], shift[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = param_at(p.w, p.param_bf16, c + j, 1.f);
+    shift[j] = param_at(p.b, p.param_bf16, c + j, 0.f);
+    if (BACKWARD && rg == 0) wts[in + j] = w[j];
+  }
+  const float inv = 1.0f / (static_cast<float>(S) * static_cast<float>(p.Cg));
+  float mean[V], rstd[V], t[V];
+  if (!BACKWARD) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      t[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < R; ++k) t[j] += io::get(rx[k], j);
+    }
+    slab_sums<V>(t, on, rg, lane, step, W, p.Cg, lds, chan[0], grp[0], nullptr);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      mean[j] = grp[0][(in + j) / p.Cg] * inv;
+      t[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const float d = io::get(rx[k], j) - mean[j];
+        t[j] = rg + k * step < S ? fmaf(d, d, t[j]) : t[j];
+      }
+    }
+    slab_sums<V>(t, on, rg, lane, step, W, p.Cg, lds, chan[0], grp[1], nullptr);
+    if (threadIdx.x < gs)
+      for (int g = threadIdx.x; g < gs; g += kSlabThreads)
+        p.stats[b * p.G + g0 + g] = make_float2(grp[0][g] * inv, 1.0f / sqrtf(fmaf(grp[1][g], inv, p.eps)));
+#pragma unroll
+    for (int j = 0; j < V; ++j) rstd[j] = w[j] / sqrtf(fmaf(grp[1][(in + j) / p.Cg], inv, p.eps));
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int r = rg + k * step;
+      float z[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[j] = fmaf(io::get(rx[k], j) - mean[j], rstd[j], shift[j]);
+      activate(z, p.act);
+      if (on && r < S) io::store(y + static_cast<int64_t>(r) * p.C, z);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float2 st = p.stats[b * p.G + g0 + (in + j) / p.Cg];
+    mean[j] = st.x;
+    rstd[j] = st.y;
+    t[j] = 0.f;
+  }
+  float dz[R][V], u[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) u[j] = 0.f;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    float z[V], xh[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      xh[j] = (io::get(rx[k], j) - mean[j]) * rstd[j];
+      z[j] = fmaf(xh[j], w[j], shift[j]);
+    }
+    slope(z, p.act);
+    const bool live = rg + k * step < S;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      dz[k][j] = live ? io::get(rd[BACKWARD ? k : 0], j) * z[j] : 0.f;
+      t[j] += dz[k][j];
+      u[j] = live ? fmaf(dz[k][j], xh[j], u[j]) : u[j];
+    }
+  }
+  slab_sums<V>(t, on, rg, lane, step, W, p.Cg, lds, chan[0], grp[0], wts);
+  slab_sums<V>(u, on, rg, lane, step, W, p.Cg, lds, chan[1], grp[1], wts);
+  for (int i = threadIdx.x; i < W; i += kSlabThreads) {
+    if (p.gb) p.gb[b * p.C + g0 * p.Cg + i] = chan[0][i];
+    if (p.gw) p.gw[b * p.C + g0 * p.Cg + i] = chan[1][i];
+  }
+  float s1[V], s2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    s1[j] = grp[0][(in + j) / p.Cg] * inv;
+    s2[j] = grp[1][(in + j) / p.Cg] * inv;
+  }
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int r = rg + k * step;
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xh = (io::get(rx[k], j) - mean[j]) * rstd[j];
+      o[j] = rstd[j] * (dz[k][j] * w[j] - s1[j] - xh * s2[j]);
+    }
+    if (on && r < S) io::store(y + static_cast<int64_t>(r) * p.C, o);
   }
 }
 
@@ -667,14 +864,14 @@ __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(NormArgs p) {
 // ---- host ------------------------------------------------------------------------------------
 
 // Vector width and the cut of [S, C] into blocks: a block covers up to 256 vectors of a row and as
-// many rows at once as its threads allow; S is cut into enough chunks to fill the GPU, none
-// shorter than 64 rows, so that the partial sums stay below a sixteenth of what is read.
+// many rows at once as its threads allow; S is cut into enough chunks to fill the GPU, none with less than
+// 64 rows or 16 for a thread, so that the partial sums stay below a sixteenth of what is read.
 void plan(NormArgs* p, int V) {
   const int vecs = p->C / V;
   p->cl = vecs < kThreads ? vecs : kThreads;
   p->cblocks = static_cast<int>(dpk_cdiv(vecs, p->cl));
   const int step = kThreads / p->cl;
-  const int64_t least = static_cast<int64_t>(step) * kRows > 64 ? static_cast<int64_t>(step) * kRows : 64;
+  const int64_t least = static_cast<int64_t>(step) * 16 > 64 ? static_cast<int64_t>(step) * 16 : 64;
   int64_t J = dpk_cdiv(kWantBlocks, p->n * p->cblocks);
   const int64_t most = dpk_cdiv(p->S, least);
   if (J > most) J = most;
@@ -689,6 +886,23 @@ int width_of(const NormArgs& p, int dtype) {
     if (p.C % V == 0 && dpk_aligned(p.x, al) && dpk_aligned(p.dy, al) && dpk_aligned(p.y, al)) return V;
   }
   return 1;
+}
+
+// Statistics per sample: the slab of whole groups a block of 512 threads can hold in registers, at most
+// 64 values a thread. False if S is too long for the narrowest one.
+bool plan_slabs(NormArgs* p, int V, int dtype, int* R) {
+  const int64_t es = static_cast<int64_t>(dpk_elsize(dtype));
+  int gs = 1;
+  while (gs < p->G && (static_cast<int64_t>(gs) * p->Cg * es < 128 || static_cast<int64_t>(gs) * p->Cg % V != 0)) ++gs;
+  const int64_t cl = static_cast<int64_t>(gs) * p->Cg / V;
+  if (cl > kSlabThreads || cl * V > kSlabWidth) return false;
+  const int64_t rows = dpk_cdiv(p->S, kSlabThreads / cl);
+  const int most = V == 8 ? 8 : 16;
+  if (rows > most) return false;
+  *R = rows <= 4 ? 4 : most;
+  p->lg = gs;
+  p->cblocks = static_cast<int>(dpk_cdiv(p->G, gs));
+  return true;
 }
 
 // Statistics per position: the widest loads for which a group's vectors fit into a wave, up to 4 a
@@ -771,6 +985,14 @@ void launch_rows(const NormArgs& p, int NI, hipStream_t s) {
   else hipLaunchKernelGGL((position_rows_kernel<T, V, 4, 1, BACKWARD>), grid, block, 0, s, p);
 }
 
+template <typename T, int V, bool BACKWARD>
+void launch_slabs(const NormArgs& p, int R, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.n * p.cblocks)), block(kSlabThreads);
+  const size_t lds = (kSlabThreads * V + 3 * p.lg * p.Cg + 2 * p.lg) * sizeof(float);
+  if (R == 4) hipLaunchKernelGGL((slab_kernel<T, V, 4, BACKWARD>), grid, block, lds, s, p);
+  else hipLaunchKernelGGL((slab_kernel<T, V, (V == 8 ? 8 : 16), BACKWARD>), grid, block, lds, s, p);
+}
+
 // Calls body(T{}, integral_constant<V>) for the tensor's type and width.
 template <typename F>
 void by_width(int dtype, int V, F&& body) {
@@ -816,6 +1038,12 @@ extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, 
     else hipLaunchKernelGGL((position_kernel<float, false>), dim3(grid), dim3(kThreads), 0, s, p);
   } else {
     V = width_of(p, dtype);
+    int R;
+    if (plan_slabs(&p, V, dtype, &R)) {
+      by_width(dtype, V, [&](auto t, auto v) { launch_slabs<decltype(t), decltype(v)::value, false>(p, R, s); });
+      DPK_LAUNCH_CHECK(fn);
+      return DPK_OK;
+    }
     plan(&p, V);
     p.part = static_cast<float2*>(ws);
     const int64_t blocks = n * p.cblocks * p.J;
@@ -862,6 +1090,12 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
     return DPK_OK;
   }
   V = width_of(p, dtype);
+  int R;
+  if (!per_position && plan_slabs(&p, V, dtype, &R)) {
+    by_width(dtype, V, [&](auto t, auto v) { launch_slabs<decltype(t), decltype(v)::value, true>(p, R, s); });
+    DPK_LAUNCH_CHECK(fn);
+    return DPK_OK;
+  }
   plan(&p, V);
   const int64_t blocks = n * p.cblocks * p.J;
   DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
