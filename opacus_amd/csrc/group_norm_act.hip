@@ -111,6 +111,21 @@ __device__ __forceinline__ float param_at(const void* p, int is_bf16, int c, flo
   return is_bf16 ? bf16_to_f32(static_cast<const bf16_t*>(p)[c]) : static_cast<const float*>(p)[c];
 }
 
+// V neighbouring parameters from channel c on, in 16-byte loads where they are aligned to that.
+template <int V>
+__device__ __forceinline__ void params_at(const void* p, int is_bf16, int c, float none, float* v) {
+  if (p && !is_bf16 && V % 4 == 0 && ((reinterpret_cast<uintptr_t>(p) >> 2) + c) % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j);
+      v[j] = q.x, v[j + (V > 1)] = q.y, v[j + 2 * (V > 2)] = q.z, v[j + 3 * (V > 3)] = q.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = param_at(p, is_bf16, c + j, none);
+}
+
 // What a thread of the streaming kernels works on: vector column c of rows r0 + rg, r0 + rg + step, ...
 struct Span {
   int64_t b, r0, r1;
@@ -243,12 +258,13 @@ __global__ __launch_bounds__(kThreads) void sample_apply_kernel(NormArgs p) {
   const T* x = static_cast<const T*>(p.x) + (s.b * p.S) * p.C + s.c;
   T* y = static_cast<T*>(p.y) + (s.b * p.S) * p.C + s.c;
   float mean[V], f[V], shift[V];
+  params_at<V>(p.w, p.param_bf16, s.c, 1.f, f);
+  params_at<V>(p.b, p.param_bf16, s.c, 0.f, shift);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const float2 st = p.stats[s.b * p.G + (s.c + j) / p.Cg];
     mean[j] = st.x;
-    f[j] = st.y * param_at(p.w, p.param_bf16, s.c + j, 1.f);
-    shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
+    f[j] *= st.y;
   }
   for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * kApplyRows) {
     typename io::raw raw[kApplyRows];
@@ -293,9 +309,9 @@ __global__ __launch_bounds__(kThreads) void channel_sums_kernel(NormArgs p) {
     for (int j = 0; j < V; ++j) {
       grp[j] = (s.c + j) / p.Cg;
       if (!PER_POSITION) st[j] = p.stats[s.b * p.G + grp[j]];
-      w[j] = param_at(p.w, p.param_bf16, s.c + j, 1.f);
-      shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
     }
+    params_at<V>(p.w, p.param_bf16, s.c, 1.f, w);
+    params_at<V>(p.b, p.param_bf16, s.c, 0.f, shift);
     for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * R) {
       typename io::raw rx[R], rd[R];
 #pragma unroll
@@ -403,9 +419,9 @@ __global__ __launch_bounds__(kThreads) void sample_dx_kernel(NormArgs p) {
     const int64_t g = s.b * p.G + (s.c + j) / p.Cg;
     st[j] = p.stats[g];
     sm[j] = p.sums[g];
-    w[j] = param_at(p.w, p.param_bf16, s.c + j, 1.f);
-    shift[j] = param_at(p.b, p.param_bf16, s.c + j, 0.f);
   }
+  params_at<V>(p.w, p.param_bf16, s.c, 1.f, w);
+  params_at<V>(p.b, p.param_bf16, s.c, 0.f, shift);
   for (int64_t r = s.r0 + s.rg; r < s.r1; r += static_cast<int64_t>(s.step) * R) {
     typename io::raw rx[R], rd[R];
 #pragma unroll
@@ -508,11 +524,11 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(NormArgs p) {
     }
   }
   float w[V], shift[V];
+  params_at<V>(p.w, p.param_bf16, c, 1.f, w);
+  params_at<V>(p.b, p.param_bf16, c, 0.f, shift);
+  if (BACKWARD && rg == 0) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    w[j] = param_at(p.w, p.param_bf16, c + j, 1.f);
-    shift[j] = param_at(p.b, p.param_bf16, c + j, 0.f);
-    if (BACKWARD && rg == 0) wts[in + j] = w[j];
+    for (int j = 0; j < V; ++j) wts[in + j] = w[j];
   }
   const float inv = 1.0f / (static_cast<float>(S) * static_cast<float>(p.Cg));
   float mean[V], rstd[V], t[V];
@@ -655,10 +671,12 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
     const int in = (i * p.lg + at) * V;
     on[i] = mine && in < p.Cg;
     c[i] = on[i] ? g * p.Cg + in : 0;
+    params_at<V>(p.w, p.param_bf16, c[i], 1.f, w + i * V);
+    params_at<V>(p.b, p.param_bf16, c[i], 0.f, shift + i * V);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      w[i * V + k] = on[i] ? param_at(p.w, p.param_bf16, c[i] + k, 1.f) : 0.f;
-      shift[i * V + k] = on[i] ? param_at(p.b, p.param_bf16, c[i] + k, 0.f) : 0.f;
+    for (int k = 0; k < V; ++k) {  // a lane without a channel adds zeros to its group's sums
+      w[i * V + k] = on[i] ? w[i * V + k] : 0.f;
+      shift[i * V + k] = on[i] ? shift[i * V + k] : 0.f;
     }
   }
   const float inv = 1.0f / static_cast<float>(p.Cg);
@@ -669,19 +687,33 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
 #pragma unroll
   for (int k = 0; k < N; ++k) A[k] = B[k] = 0.f;
 
-  for (int64_t r = r0 + wave * R; r < r1; r += kWaves * R) {
-    typename io::raw rx[R][NI], rd[R][NI];
+  typename io::raw nx[R][NI], nd[BACKWARD ? R : 1][NI];
+  const auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        rx[q][i] = rd[q][i] = typename io::raw();
+        nx[q][i] = typename io::raw();
+        if (BACKWARD) nd[BACKWARD ? q : 0][i] = typename io::raw();
         if (on[i] && r + q < r1) {
-          rx[q][i] = io::load(x + (r + q) * p.C + c[i]);
-          if (BACKWARD) rd[q][i] = io::load(dy + (r + q) * p.C + c[i]);
+          nx[q][i] = io::load(x + (r + q) * p.C + c[i]);
+          if (BACKWARD) nd[BACKWARD ? q : 0][i] = io::load(dy + (r + q) * p.C + c[i]);
         }
       }
     }
+  };
+  fetch(r0 + wave * R);
+  for (int64_t r = r0 + wave * R; r < r1; r += kWaves * R) {
+    typename io::raw rx[R][NI], rd[BACKWARD ? R : 1][NI];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        rx[q][i] = nx[q][i];
+        if (BACKWARD) rd[BACKWARD ? q : 0][i] = nd[BACKWARD ? q : 0][i];
+      }
+    }
+    fetch(r + kWaves * R);  // the next rows, under this batch's arithmetic
     float mean[R], rstd[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -739,7 +771,7 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
 #pragma unroll
           for (int k = 0; k < V; ++k) {
             // a row behind the last one has dy = 0, but its slope may not be a number times zero
-            const float dz = r + q < r1 ? io::get(rd[q][i], k) * z[k] : 0.f;
+            const float dz = r + q < r1 ? io::get(rd[BACKWARD ? q : 0][i], k) * z[k] : 0.f;
             A[i * V + k] += dz;
             B[i * V + k] = r + q < r1 ? fmaf(dz, xh[q][i * V + k], B[i * V + k]) : B[i * V + k];
             d[q][i * V + k] = dz * w[i * V + k];
@@ -852,6 +884,7 @@ __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(NormArgs p) {
   const int64_t b = i / p.C;
   const float2* part = p.part + b * p.J * p.C + (i - b * p.C);
   float A = 0.f, B = 0.f;
+#pragma unroll 8
   for (int j = 0; j < p.J; ++j) {
     const float2 v = part[static_cast<int64_t>(j) * p.C];
     A += v.x;
@@ -863,21 +896,29 @@ __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(NormArgs p) {
 
 // ---- host ------------------------------------------------------------------------------------
 
-// Vector width and the cut of [S, C] into blocks: a block covers up to 256 vectors of a row and as
-// many rows at once as its threads allow; S is cut into enough chunks to fill the GPU, none with less than
-// 64 rows or 16 for a thread, so that the partial sums stay below a sixteenth of what is read.
-void plan(NormArgs* p, int V) {
+// The cut of [S, C] into blocks: a block covers up to 256 vectors of a row and as many rows at once as
+// its threads allow; S is cut into enough chunks to fill the GPU. `sums`: the chunks leave partial sums
+// of 8 bytes a channel, and none has less than 64 rows, or 8 for a thread.
+void plan(NormArgs* p, int V, bool sums) {
   const int vecs = p->C / V;
   p->cl = vecs < kThreads ? vecs : kThreads;
   p->cblocks = static_cast<int>(dpk_cdiv(vecs, p->cl));
   const int step = kThreads / p->cl;
-  const int64_t least = static_cast<int64_t>(step) * 16 > 64 ? static_cast<int64_t>(step) * 16 : 64;
+  int64_t least = static_cast<int64_t>(step) * (sums ? 8 : kApplyRows);
+  if (sums && least < 64) least = 64;
   int64_t J = dpk_cdiv(kWantBlocks, p->n * p->cblocks);
   const int64_t most = dpk_cdiv(p->S, least);
   if (J > most) J = most;
   if (J < 1) J = 1;
   p->chunk = dpk_cdiv(p->S, J);
   p->J = static_cast<int>(dpk_cdiv(p->S, p->chunk));
+}
+
+int grid_of(const char* fn, const NormArgs& p, dim3* grid) {
+  const int64_t blocks = p.n * p.cblocks * p.J;
+  DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+  *grid = dim3(static_cast<unsigned>(blocks));
+  return DPK_OK;
 }
 
 int width_of(const NormArgs& p, int dtype) {
@@ -934,7 +975,7 @@ size_t part_bytes(int64_t n, int64_t S, int64_t C) {
     if (C % V) break;
     NormArgs p = {};
     p.n = n, p.S = S, p.C = static_cast<int>(C);
-    plan(&p, V);
+    plan(&p, V, true);
     const size_t need = static_cast<size_t>(n) * p.J * C * sizeof(float2);
     if (need > most) most = need;
   }
@@ -1044,15 +1085,16 @@ extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, 
       DPK_LAUNCH_CHECK(fn);
       return DPK_OK;
     }
-    plan(&p, V);
+    plan(&p, V, true);
     p.part = static_cast<float2*>(ws);
-    const int64_t blocks = n * p.cblocks * p.J;
-    DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
-    const dim3 grid(static_cast<unsigned>(blocks));
+    dim3 grid;
+    if (int rc = grid_of(fn, p, &grid)) return rc;
     by_width(dtype, V, [&](auto t, auto v) {
       hipLaunchKernelGGL((sample_stat_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0, s, p);
     });
     hipLaunchKernelGGL(sample_stat_merge_kernel, dim3(static_cast<unsigned>(n * groups)), dim3(kThreads), 0, s, p);
+    plan(&p, V, false);
+    if (int rc = grid_of(fn, p, &grid)) return rc;
     by_width(dtype, V, [&](auto t, auto v) {
       hipLaunchKernelGGL((sample_apply_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0, s, p);
     });
@@ -1096,10 +1138,9 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
     DPK_LAUNCH_CHECK(fn);
     return DPK_OK;
   }
-  plan(&p, V);
-  const int64_t blocks = n * p.cblocks * p.J;
-  DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
-  const dim3 grid(static_cast<unsigned>(blocks));
+  plan(&p, V, true);
+  dim3 grid;
+  if (int rc = grid_of(fn, p, &grid)) return rc;
   float2* groups_ws = reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(n, S, C));
   if (per_position) {
     p.stats = groups_ws;
@@ -1118,6 +1159,8 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
       hipLaunchKernelGGL((channel_sums_kernel<decltype(t), decltype(v)::value, false>), grid, dim3(kThreads), 0, s, p);
     });
     hipLaunchKernelGGL(sample_grad_merge_kernel, dim3(static_cast<unsigned>(n * groups)), dim3(kThreads), 0, s, p);
+    plan(&p, V, false);
+    if (int rc = grid_of(fn, p, &grid)) return rc;
     by_width(dtype, V, [&](auto t, auto v) {
       hipLaunchKernelGGL((sample_dx_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0, s, p);
     });

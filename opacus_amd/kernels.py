@@ -888,15 +888,22 @@ def layer_norm_grad_sample(
 
 
 # ---- gated linear recurrence ----------------------------------------------------------
-@contextmanager
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device around a launch: a kernel goes to the current device, and
-    the tensors may live on another one."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        yield
+def _launch(name: str, dev: torch.device, *args) -> None:
+    """Calls entry point ``name`` with ``args`` (addresses as plain integers) and torch's current stream
+    of ``dev``. A kernel goes to the current device, so that is made ``dev`` around the call where it is
+    another one. The usual case takes no context manager: for the one-token calls the host's time is
+    the time."""
+    if _TIMING is None and _raw_stream is not None and dev.index == torch._C._cuda_getDevice():
+        status = getattr(lib(), name)(*args, _raw_stream(dev.index))
     else:
-        with torch.cuda.device(dev):
-            yield
+        with torch.cuda.device(dev), _timed(name[4:], dev):
+            status = getattr(lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if status != 0:
+        check(name, status)
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _gates_layout(gates: torch.Tensor, D: int) -> Tuple[torch.Tensor, int, int]:
@@ -960,14 +967,11 @@ def gated_scan(
     gates, sn, st = _gates_layout(gates, D)
     L = lib()
     ws, wsb = _ws(L.dpk_gated_scan_workspace_bytes(n, T, D), dev)
-    with _on(dev), _timed("gated_scan", dev):
-        check(
-            "dpk_gated_scan",
-            L.dpk_gated_scan(
-                _ptr(gates), _code(gates), _ptr(decay), _code(decay), _ptr(state), _ptr(lengths), _ptr(out), _ptr(last),
-                _ptr(kept), n, T, D, sn, st, int(bool(reverse)), _ptr(ws), wsb, _stream(dev),
-            ),
-        )
+    _launch(
+        "dpk_gated_scan", dev,
+        _at(gates), _code(gates), _at(decay), _code(decay), _at(state), _at(lengths), _at(out), _at(last),
+        _at(kept), n, T, D, sn, st, int(bool(reverse)), _at(ws), wsb,
+    )
     return out, last, kept
 
 
@@ -1003,15 +1007,12 @@ def gated_scan_backward(
     grad_out = _dense(grad_out)
     L = lib()
     ws, wsb = _ws(L.dpk_gated_scan_workspace_bytes(n, T, D), dev)
-    with _on(dev), _timed("gated_scan_backward", dev):
-        check(
-            "dpk_gated_scan_backward",
-            L.dpk_gated_scan_backward(
-                _ptr(gates), _code(gates), _ptr(decay), _code(decay), _ptr(kept), _ptr(lengths), _ptr(grad_out),
-                _ptr(grad_last), _ptr(grad_gates), _ptr(grad_decay), _ptr(grad_state), n, T, D, sn, st,
-                int(bool(reverse)), _ptr(ws), wsb, _stream(dev),
-            ),
-        )
+    _launch(
+        "dpk_gated_scan_backward", dev,
+        _at(gates), _code(gates), _at(decay), _code(decay), _at(kept), _at(lengths), _at(grad_out),
+        _at(grad_last), _at(grad_gates), _at(grad_decay), _at(grad_state), n, T, D, sn, st,
+        int(bool(reverse)), _at(ws), wsb,
+    )
     return grad_gates, grad_decay, grad_state
 
 
@@ -1030,14 +1031,11 @@ def gated_scan_step(gates: torch.Tensor, decay: torch.Tensor, state: torch.Tenso
         return out
     if gates.stride(1) != 1 or gates.stride(0) < 0:
         gates = gates.contiguous()
-    with _on(dev), _timed("gated_scan_step", dev):
-        check(
-            "dpk_gated_scan_step",
-            lib().dpk_gated_scan_step(
-                _ptr(gates), _code(gates), _ptr(decay), _code(decay), _ptr(state), _ptr(out), n, D,
-                gates.stride(0) if n > 1 else 3 * D, _stream(dev),
-            ),
-        )
+    _launch(
+        "dpk_gated_scan_step", dev,
+        _at(gates), _code(gates), _at(decay), _code(decay), _at(state), _at(out), n, D,
+        gates.stride(0) if n > 1 else 3 * D,
+    )
     torch.autograd.graph.increment_version(state)
     return out
 
@@ -1089,14 +1087,11 @@ def group_norm_act(
         return y, stats
     L = lib()
     ws, wsb = _ws(L.dpk_group_norm_act_workspace_bytes(n, S, C, num_groups, int(bool(per_position))), dev)
-    with _on(dev), _timed("group_norm_act", dev):
-        check(
-            "dpk_group_norm_act",
-            L.dpk_group_norm_act(
-                _ptr(x), _code(x), _ptr(weight), _ptr(bias), pcode, _ptr(y), _ptr(stats), n, S, C, num_groups, float(eps),
-                _lib.DPK_ACT[activation], int(bool(per_position)), _ptr(ws), wsb, _stream(dev),
-            ),
-        )
+    _launch(
+        "dpk_group_norm_act", dev,
+        _at(x), _code(x), _at(weight), _at(bias), pcode, _at(y), _at(stats), n, S, C, num_groups, float(eps),
+        _lib.DPK_ACT[activation], int(bool(per_position)), _at(ws), wsb,
+    )
     return y, stats
 
 
@@ -1136,15 +1131,12 @@ def group_norm_act_backward(
     grad_b = torch.empty((n, C), dtype=torch.float32, device=dev)
     L = lib()
     ws, wsb = _ws(L.dpk_group_norm_act_workspace_bytes(n, S, C, num_groups, int(bool(per_position))), dev)
-    with _on(dev), _timed("group_norm_act_backward", dev):
-        check(
-            "dpk_group_norm_act_backward",
-            L.dpk_group_norm_act_backward(
-                _ptr(x), _ptr(grad_out), _code(x), _ptr(weight), _ptr(bias), pcode, _ptr(stats), _ptr(grad_x), _ptr(grad_w),
-                _ptr(grad_b), n, S, C, num_groups, float(eps), _lib.DPK_ACT[activation], int(bool(per_position)),
-                _ptr(ws), wsb, _stream(dev),
-            ),
-        )
+    _launch(
+        "dpk_group_norm_act_backward", dev,
+        _at(x), _at(grad_out), _code(x), _at(weight), _at(bias), pcode, _at(stats), _at(grad_x), _at(grad_w),
+        _at(grad_b), n, S, C, num_groups, float(eps), _lib.DPK_ACT[activation], int(bool(per_position)),
+        _at(ws), wsb,
+    )
     return grad_x, grad_w, grad_b
 
 
