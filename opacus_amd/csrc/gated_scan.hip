@@ -6,7 +6,7 @@
 //
 // The recurrence is a composition of affine maps h -> A h + B, so T is cut at will. A block takes one
 // tile of positions for 16 * V channels of a sample: every thread runs K positions of its channels in
-// registers, the 16 time groups exchange their (A, B) through LDS, and the tiles of a row pass
+// registers, the block's time groups exchange their (A, B) through LDS, and the tiles of a row pass
 // the state on in one launch (see "the chain" below), so every input is read once and every output
 // written once. What is folded, and in which order, depends on sizes alone: the same bits on every run.
 //
@@ -24,14 +24,14 @@
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kCL = 32;                  // lanes across channels
-constexpr int kTG = kThreads / kCL;      // time groups of a block
+constexpr int kThreads = 256;            // of the forward kernel and the small ones
+constexpr int kBwdThreads = 256;
+constexpr int kCL = 32;                  // lanes across channels: a wave holds two time groups
 constexpr int kChunk = DPK_SCAN_CHUNK;   // positions between kept states
 constexpr int kFwdK = 16;                // positions per thread
 constexpr int kBwdK = 8;
-constexpr int kFwdTile = kTG * kFwdK;    // 128
-constexpr int kBwdTile = kTG * kBwdK;    // 64
+constexpr int kFwdTile = kThreads / kCL * kFwdK;     // 128
+constexpr int kBwdTile = kBwdThreads / kCL * kBwdK;  // 64
 static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0 && kChunk % kFwdK == 0, "tiles start at kept states");
 // Byte offsets inside a tile are 32 bits wide.
 constexpr int64_t kMaxStride = (1LL << 31) / (kFwdTile * 4) - 1;
@@ -140,31 +140,32 @@ __device__ __forceinline__ int drawn_tile(const int* lds) {
   return __builtin_amdgcn_readfirstlane(*lds);
 }
 
-// Tile t's own map (TA, TB), for the tiles behind it in its run.
+// Tile t's own map (TA, TB), for the tiles behind it in its run. `owner`: the lanes that hold it.
 template <int V>
-__device__ __forceinline__ void publish_map(const Chain& ch, int64_t row, int t, int cl, int tg, const float (&TA)[V],
+__device__ __forceinline__ void publish_map(const Chain& ch, int64_t row, int t, int cl, bool owner, const float (&TA)[V],
                                             const float (&TB)[V]) {
-  if (tg == 0 && t + 1 < ch.tiles && t % kRun + 1 < kRun) {
+  if (owner && t + 1 < ch.tiles && t % kRun + 1 < kRun) {
     uint64_t* w = ch.maps + (row * ch.tiles + t) * (kCL * V) + cl * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) publish(w + j, TA[j], TB[j]);
   }
 }
-// The state that enters tile t, in `in`, which holds the row's first state. All threads call it;
-// lds_m: [2][kRun][W], lds_s: [W], used by nothing else.
-template <int V>
-__device__ __forceinline__ void state_before(const Chain& ch, int64_t row, int t, int cl, int tg, const float (&TA)[V],
-                                             const float (&TB)[V], float (&in)[V], float* lds_m, float* lds_s) {
+// The state that enters tile t, in `in`, which holds the row's first state. All threads call it, TG
+// time groups; lds_m: [2][kRun][W], lds_s: [W], used by nothing else.
+template <int V, int TG>
+__device__ __forceinline__ void state_before(const Chain& ch, int64_t row, int t, int cl, int tg, bool owner,
+                                             const float (&TA)[V], const float (&TB)[V], float (&in)[V], float* lds_m,
+                                             float* lds_s) {
   constexpr int W = kCL * V;
   const int run = t / kRun, k = t - run * kRun;
   if (t > 0) {
     float x[V], y[V];
-    for (int g = tg; g < k; g += kTG) {
+    for (int g = tg; g < k; g += TG) {
       await<V>(ch.maps + (row * ch.tiles + run * kRun + g) * W + cl * V, x, y);
 #pragma unroll
       for (int j = 0; j < V; ++j) lds_m[g * W + cl * V + j] = x[j], lds_m[(kRun + g) * W + cl * V + j] = y[j];
     }
-    if (tg == kTG - 1 && run > 0) {
+    if (tg == TG - 1 && run > 0) {
       await<V>(ch.states + (row * ch.runs + run) * W + cl * V, x, y);
 #pragma unroll
       for (int j = 0; j < V; ++j) lds_s[cl * V + j] = y[j];
@@ -179,7 +180,7 @@ __device__ __forceinline__ void state_before(const Chain& ch, int64_t row, int t
       for (int j = 0; j < V; ++j) in[j] = fmaf(lds_m[g * W + cl * V + j], in[j], lds_m[(kRun + g) * W + cl * V + j]);
     }
   }
-  if (tg == 0 && t + 1 < ch.tiles && k + 1 == kRun) {
+  if (owner && t + 1 < ch.tiles && k + 1 == kRun) {
     uint64_t* w = ch.states + (row * ch.runs + run + 1) * W + cl * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) publish(w + j, 0.f, fmaf(TA[j], in[j], TB[j]));
@@ -280,23 +281,25 @@ __device__ __forceinline__ Tile tile_of(int64_t T, int64_t len, int64_t s0, int 
   return t;
 }
 
-// prefix = the composition of the groups before tg, total = of all kTG, in the order of the scan
-// (BACK: from the last group to the first). The wave's own groups are the only ones at which
-// lanes differ, so the rest is folded without selects.
-template <int V, bool BACK>
-__device__ __forceinline__ void fold_groups(const float (*la)[kCL * V], const float (*lb)[kCL * V], int cl, int tg,
-                                            float (&PA)[V], float (&PB)[V], float (&TA)[V], float (&TB)[V]) {
+// The value of the wave's other time group.
+template <int V>
+__device__ __forceinline__ void other_group(const float (&v)[V], float (&o)[V]) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) TA[j] = PA[j] = 1.f, TB[j] = PB[j] = 0.f;
-#pragma unroll 2  // (all eight unrolled, the LDS reads in flight alone would cost a wave of occupancy)
-  for (int i = 0; i < kTG; ++i) {
-    const int g = BACK ? kTG - 1 - i : i;
+  for (int j = 0; j < V; ++j) o[j] = __shfl_xor(v[j], 32, DPK_WAVE);
+}
+// P = the composition of the waves [from, to) in steps of `step`, whose maps lie in LDS. The bounds
+// are the same for the whole wave, so nothing is folded that a lane does not need.
+template <int V>
+__device__ __forceinline__ void fold_waves(const float (*la)[kCL * V], const float (*lb)[kCL * V], int cw, int from, int to,
+                                           int step, float (&PA)[V], float (&PB)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) PA[j] = 1.f, PB[j] = 0.f;
+  for (int w = from; w != to; w += step) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (g == tg) PA[j] = TA[j], PB[j] = TB[j];
-      const float ga = la[g][cl * V + j];
-      TB[j] = fmaf(ga, TB[j], lb[g][cl * V + j]);
-      TA[j] *= ga;
+      const float a = la[w][cw + j];
+      PB[j] = fmaf(a, PB[j], lb[w][cw + j]);
+      PA[j] *= a;
     }
   }
 }
@@ -306,8 +309,10 @@ template <typename T, int V, bool FULL>
 __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
                                          const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
-  constexpr int W = kCL * V, K = kFwdK, E = sizeof(T);
+  constexpr int W = kCL * V, K = kFwdK, E = sizeof(T), kWaves = kThreads / DPK_WAVE;
   const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / DPK_WAVE);
+  const bool late = tg & 1;  // the later one of the wave's two time groups
   const int cw = cl * V, c = static_cast<int>(cb) * W + cw;
   const bool on = FULL || c < p.D;
   const int D = static_cast<int>(p.D), st = static_cast<int>(p.st);
@@ -349,19 +354,31 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
       B[j] = fmaf(a[k][j], B[j], u[k][j]);
     }
   }
+  float Ao[V], Bo[V], TA[V], TB[V], PA[V], PB[V];
+  other_group<V>(A, Ao);
+  other_group<V>(B, Bo);
 #pragma unroll
-  for (int j = 0; j < V; ++j) lds_a[tg][cw + j] = A[j], lds_b[tg][cw + j] = B[j];
+  for (int j = 0; j < V; ++j) {
+    TA[j] = A[j] * Ao[j];
+    TB[j] = late ? fmaf(A[j], Bo[j], B[j]) : fmaf(Ao[j], B[j], Bo[j]);
+    if (!late) lds_a[wave][cw + j] = TA[j], lds_b[wave][cw + j] = TB[j];
+  }
   __syncthreads();
-  float TA[V], TB[V], PA[V], PB[V];
-  fold_groups<V, false>(lds_a, lds_b, cl, tg, PA, PB, TA, TB);
-  publish_map<V>(p.ch, r, t, cl, tg, TA, TB);
-  state_before<V>(p.ch, r, t, cl, tg, TA, TB, h, lds_m, lds_s);
-  if (on && tg == 0 && t + 1 == p.ch.tiles) {
+  fold_waves<V>(lds_a, lds_b, cw, 0, wave, 1, PA, PB);
+  const bool owner = wave == kWaves - 1 && !late;
+#pragma unroll
+  for (int j = 0; j < V; ++j) TB[j] = fmaf(TA[j], PB[j], TB[j]), TA[j] *= PA[j];  // the tile's map, in the last wave
+  publish_map<V>(p.ch, r, t, cl, owner, TA, TB);
+  state_before<V, kThreads / kCL>(p.ch, r, t, cl, tg, owner, TA, TB, h, lds_m, lds_s);
+  if (on && owner && t + 1 == p.ch.tiles) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.last[row + j] = fmaf(TA[j], h[j], TB[j]);
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) h[j] = fmaf(PA[j], h[j], PB[j]);
+  for (int j = 0; j < V; ++j) {
+    h[j] = fmaf(PA[j], h[j], PB[j]);
+    h[j] = late ? fmaf(Ao[j], h[j], Bo[j]) : h[j];
+  }
   if (!on || tg * K >= tl.count) return;
   if (p.kept && (tg * K) % kChunk == 0) {
     const int64_t s = static_cast<int64_t>(t) * kFwdTile + tg * K;
@@ -386,9 +403,9 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
 // One block: one tile of 128 positions of 32 * V channels of one sample.
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_kernel(ScanArgs p) {
-  constexpr int W = kCL * V;
-  __shared__ float lds_a[kTG][W];
-  __shared__ float lds_b[kTG][W];
+  constexpr int W = kCL * V, kWaves = kThreads / DPK_WAVE;
+  __shared__ float lds_a[kWaves][W];
+  __shared__ float lds_b[kWaves][W];
   __shared__ float lds_m[2 * kRun * W];
   __shared__ float lds_s[W];
   __shared__ int lds_t;
@@ -407,11 +424,13 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
                                          const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float (*lds_g)[kCL * V],
                                          float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
-  constexpr int W = kCL * V, K = kBwdK, E = sizeof(T);
+  constexpr int W = kCL * V, K = kBwdK, E = sizeof(T), kWaves = kBwdThreads / DPK_WAVE;
   const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
   const int cw = cl * V, c = static_cast<int>(cb) * W + cw;
   const bool on = FULL || c < p.D;
   const int D = static_cast<int>(p.D), st = static_cast<int>(p.st);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / DPK_WAVE);
+  const bool late = tg & 1;  // the later one of the wave's two time groups
   const int tile = p.ch.tiles - 1 - t;
   const T* gx = static_cast<const T*>(p.gates) + b * p.sn + tl.low * p.st + cb * W;
   const T *gr = gx + D, *gi = gr + D;
@@ -471,21 +490,34 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
 #pragma unroll
     for (int j = 0; j < V; ++j) G[j] = a[k][j] * (io::get(rd[k], j) + G[j]);
   }
+  // Ao, Bo, Go: the other group's; T: the pair's, then (in wave 0, the first in time) the tile's
+  float Ao[V], Bo[V], Go[V], TA[V], TG[V], PA[V], PG[V];
+  other_group<V>(A, Ao);
+  other_group<V>(B, Bo);
+  other_group<V>(G, Go);
 #pragma unroll
-  for (int j = 0; j < V; ++j) lds_a[tg][cw + j] = A[j], lds_b[tg][cw + j] = B[j], lds_g[tg][cw + j] = G[j];
-  __syncthreads();
-  float TA[V], TG[V], PA[V], PG[V];
-  fold_groups<V, true>(lds_a, lds_g, cl, tg, PA, PG, TA, TG);
-  publish_map<V>(p.ch, r, t, cl, tg, TA, TG);
-  // the states inside the tile, while the words of the chain are on their way
-#pragma unroll 2
-  for (int o = 0; o < kTG; ++o) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float n = fmaf(lds_a[o][cw + j], h[j], lds_b[o][cw + j]);
-      h[j] = o < tg ? n : h[j];
+  for (int j = 0; j < V; ++j) {
+    TA[j] = A[j] * Ao[j];
+    TG[j] = late ? fmaf(Ao[j], G[j], Go[j]) : fmaf(A[j], Go[j], G[j]);
+    if (!late) {
+      lds_a[wave][cw + j] = TA[j];
+      lds_b[wave][cw + j] = fmaf(Ao[j], B[j], Bo[j]);
+      lds_g[wave][cw + j] = TG[j];
     }
   }
+  __syncthreads();
+  fold_waves<V>(lds_a, lds_g, cw, kWaves - 1, wave, -1, PA, PG);
+  const bool owner = wave == 0 && !late;
+#pragma unroll
+  for (int j = 0; j < V; ++j) TG[j] = fmaf(TA[j], PG[j], TG[j]), TA[j] *= PA[j];
+  publish_map<V>(p.ch, r, t, cl, owner, TA, TG);
+  // the states inside the tile, while the words of the chain are on their way
+  for (int w = 0; w < wave; ++w) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = fmaf(lds_a[w][cw + j], h[j], lds_b[w][cw + j]);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) h[j] = late ? fmaf(Ao[j], h[j], Bo[j]) : h[j];
   // The products below are formed again, not kept from the first half: the empty asm makes the
   // compiler take the factors as new values, which keeps a thread's registers down.
 #pragma unroll
@@ -504,13 +536,16 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
       h[j] = fmaf(a[k][j], h[j], ms[k][j] * io::get(rx[k], j));
     }
   }
-  state_before<V>(p.ch, r, t, cl, tg, TA, TG, g, lds_m, lds_s);
-  if (on && tg == 0 && p.dstate && tile == 0) {
+  state_before<V, kBwdThreads / kCL>(p.ch, r, t, cl, tg, owner, TA, TG, g, lds_m, lds_s);
+  if (on && owner && p.dstate && tile == 0) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.dstate[row + j] = fmaf(TA[j], g[j], TG[j]);
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) g[j] = fmaf(PA[j], g[j], PG[j]);
+  for (int j = 0; j < V; ++j) {
+    g[j] = fmaf(PA[j], g[j], PG[j]);
+    g[j] = late ? g[j] : fmaf(Ao[j], g[j], Go[j]);
+  }
   T* dg = static_cast<T*>(p.dgates) + (b * p.T + tl.low) * 3 * p.D + cb * W;
   T *dr = dg + D, *di = dr + D;
 #pragma unroll
@@ -541,30 +576,35 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
     }
   }
   if (!p.dlam) return;
-  // sum_t w of the tile over the time groups, in order
+  // sum_t of the tile over the time groups, in order
+  float other[V];
+  other_group<V>(acc, other);
   __syncthreads();
+  if (!late) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) lds_g[tg][cw + j] = acc[j];
+    for (int j = 0; j < V; ++j) lds_g[wave][cw + j] = acc[j] + other[j];
+  }
   __syncthreads();
-  if (on && tg == 0) {
+  if (on && owner) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float sum = 0.f;
 #pragma unroll
-      for (int o = 0; o < kTG; ++o) sum += lds_g[o][cw + j];
-      // sigma(lam) / softplus(lam) times the -softplus(lam) that v lacks of w; lam is short of one here
-      p.dlam[tile * nD + row + j] = -sum * -expm1f(-sp[j]);
+      for (int w = 0; w < kWaves; ++w) sum += lds_g[w][cw + j];
+      // v lacks the factor -softplus(lam) of w, and dlam = sigma(lam) / softplus(lam) sum_t w;
+      // sigma(lam) = 1 - exp(-softplus(lam))
+      p.dlam[tile * nD + row + j] = expm1f(-sp[j]) * sum;
     }
   }
 }
 
 // One block: one tile of 64 positions, from the row's last to its first.
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads, 3) void scan_bwd_kernel(ScanBwdArgs p) {
-  constexpr int W = kCL * V;
-  __shared__ float lds_a[kTG][W];
-  __shared__ float lds_b[kTG][W];
-  __shared__ float lds_g[kTG][W];
+__global__ __launch_bounds__(kBwdThreads, 3) void scan_bwd_kernel(ScanBwdArgs p) {
+  constexpr int W = kCL * V, kWaves = kBwdThreads / DPK_WAVE;
+  __shared__ float lds_a[kWaves][W];
+  __shared__ float lds_b[kWaves][W];
+  __shared__ float lds_g[kWaves][W];
   __shared__ float lds_m[2 * kRun * W];
   __shared__ float lds_s[W];
   __shared__ int lds_t;
@@ -759,7 +799,7 @@ extern "C" int dpk_gated_scan_backward(const void* gates, int dtype, const void*
   char* behind = chain_of(&p.ch, n, D, V, tiles, ws, s);
   if (tiles > 1 && grad_decay) p.dlam = reinterpret_cast<float*>(behind);
   const dim3 grid(static_cast<unsigned>(p.ch.rows * tiles));
-#define DPK_SCAN_BWD(TT, VV) hipLaunchKernelGGL((scan_bwd_kernel<TT, VV>), grid, dim3(kThreads), 0, s, p)
+#define DPK_SCAN_BWD(TT, VV) hipLaunchKernelGGL((scan_bwd_kernel<TT, VV>), grid, dim3(kBwdThreads), 0, s, p)
   if (dtype == DPK_BF16) {
     if (V == 2) DPK_SCAN_BWD(bf16_t, 2);
     else DPK_SCAN_BWD(bf16_t, 1);
