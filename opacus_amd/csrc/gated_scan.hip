@@ -28,11 +28,10 @@ constexpr int kThreads = 256;            // of the forward kernel and the small 
 constexpr int kBwdThreads = 256;
 constexpr int kCL = 32;                  // lanes across channels: a wave holds two time groups
 constexpr int kChunk = DPK_SCAN_CHUNK;   // positions between kept states
-constexpr int kFwdK = 16;                // positions per thread
-constexpr int kBwdK = 8;
-constexpr int kFwdTile = kThreads / kCL * kFwdK;     // 128
+constexpr int kBwdK = 8;                 // positions per thread
 constexpr int kBwdTile = kBwdThreads / kCL * kBwdK;  // 64
-static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0 && kChunk % kFwdK == 0, "tiles start at kept states");
+constexpr int kFwdTile = 128;            // forward: 16 positions per thread, or 8 where T is 64 at most
+static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0, "tiles start at kept states");
 // Byte offsets inside a tile are 32 bits wide.
 constexpr int64_t kMaxStride = (1LL << 31) / (kFwdTile * 4) - 1;
 
@@ -305,11 +304,11 @@ __device__ __forceinline__ void fold_waves(const float (*la)[kCL * V], const flo
 }
 
 // FULL: every position and channel of the tile is live.
-template <typename T, int V, bool FULL>
+template <typename T, int V, int K, bool FULL>
 __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
                                          const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
-  constexpr int W = kCL * V, K = kFwdK, E = sizeof(T), kWaves = kThreads / DPK_WAVE;
+  constexpr int W = kCL * V, E = sizeof(T), kWaves = kThreads / DPK_WAVE, TILE = kThreads / kCL * K;
   const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / DPK_WAVE);
   const bool late = tg & 1;  // the later one of the wave's two time groups
@@ -381,7 +380,7 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
   }
   if (!on || tg * K >= tl.count) return;
   if (p.kept && (tg * K) % kChunk == 0) {
-    const int64_t s = static_cast<int64_t>(t) * kFwdTile + tg * K;
+    const int64_t s = static_cast<int64_t>(t) * TILE + tg * K;
     vec_io<float, V>::store(p.kept + (b * ((p.T + kChunk - 1) / kChunk) + s / kChunk) * p.D + c, h);
   }
   T* out = static_cast<T*>(p.out) + (b * p.T + tl.low) * p.D + cb * W;
@@ -400,10 +399,11 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
   }
 }
 
-// One block: one tile of 128 positions of 32 * V channels of one sample.
-template <typename T, int V>
+// One block: one tile of 8 * K positions of 32 * V channels of one sample.
+template <typename T, int V, int K>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_kernel(ScanArgs p) {
-  constexpr int W = kCL * V, kWaves = kThreads / DPK_WAVE;
+  constexpr int W = kCL * V, kWaves = kThreads / DPK_WAVE, TILE = kThreads / kCL * K;
+  static_assert(TILE % kChunk == 0 && kChunk % K == 0, "a time group starts where a state is kept");
   __shared__ float lds_a[kWaves][W];
   __shared__ float lds_b[kWaves][W];
   __shared__ float lds_m[2 * kRun * W];
@@ -414,9 +414,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_ker
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
   const int t = drawn_tile(&lds_t);
-  const Tile tl = tile_of<kFwdTile>(p.T, live_length(p.lengths, b, p.T), static_cast<int64_t>(t) * kFwdTile, p.reverse);
-  if (tl.hi - tl.lo == kFwdTile && (cb + 1) * W <= p.D) fwd_tile<T, V, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
-  else fwd_tile<T, V, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
+  const Tile tl = tile_of<TILE>(p.T, live_length(p.lengths, b, p.T), static_cast<int64_t>(t) * TILE, p.reverse);
+  if (tl.hi - tl.lo == TILE && (cb + 1) * W <= p.D) fwd_tile<T, V, K, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
+  else fwd_tile<T, V, K, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
 }
 
 template <typename T, int V, bool FULL>
@@ -760,7 +760,13 @@ extern "C" int dpk_gated_scan(const void* gates, int dtype, const void* decay, i
                 decay_dtype == DPK_BF16, reverse, {}};
   chain_of(&p.ch, n, D, V, tiles, ws, s);
   const dim3 grid(static_cast<unsigned>(p.ch.rows * tiles));
-#define DPK_SCAN_FWD(TT, VV) hipLaunchKernelGGL((scan_fwd_kernel<TT, VV>), grid, dim3(kThreads), 0, s, p)
+// 16 positions a thread; 8 where a tile of 128 would be half empty (256 x 64 x 2048 bf16: 92 us with 16,
+// 56 with 8; 128 x 128 x 2048: 48 with 16, 63 with 8; 4 x 4096 x 2048: 57 and 69)
+#define DPK_SCAN_FWD(TT, VV)                                                                                           \
+  do {                                                                                                                 \
+    if (T <= kChunk) hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 8>), grid, dim3(kThreads), 0, s, p);                  \
+    else hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 16>), grid, dim3(kThreads), 0, s, p);                             \
+  } while (0)
   if (dtype == DPK_BF16) {
     if (V == 2) DPK_SCAN_FWD(bf16_t, 2);
     else DPK_SCAN_FWD(bf16_t, 1);
