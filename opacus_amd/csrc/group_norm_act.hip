@@ -98,7 +98,8 @@ struct NormArgs {
   int64_t n, S;
   int C, G, Cg;
   int cl;               // vectors of a row that a block covers
-  int lg;               // lanes of a group (statistics per position)
+  int lg;               // lanes of a group (statistics per position), or groups of a slab
+  int wide;             // groups of a row that a wave takes, a power of two
   int cblocks;          // blocks along a row
   int J;                // row chunks of a sample
   int64_t chunk;        // rows of one
@@ -622,9 +623,10 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(NormArgs p) {
 // ---- statistics per position: the groups of a row side by side in the lanes of a wave ------------
 //
 // A group takes `lg` lanes (the least power of two that holds its vectors, NI vectors a lane where 64
-// lanes are not enough), a wave 64 / lg groups of one row and the same groups of the next rows, so a
-// row's sums are a few lane exchanges, and the columns a lane holds never change: weight and
-// bias stay in registers, and so do the per-sample sums along the rows. Nothing is read twice.
+// lanes are not enough), a wave `wide` groups of a row and, where a row has fewer, as many rows side by
+// side as fill it; then the same groups of the next rows. A row's sums are a few lane exchanges, and
+// the columns a lane holds never change: weight and bias stay in registers, and so do the
+// per-sample sums along the rows. Nothing is read twice.
 
 // v[i] = sum of v[i] over the lg lanes of the group, in all of them.
 template <int R>
@@ -661,7 +663,8 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
   const int64_t b = BACKWARD ? rest / p.J : 0, j = BACKWARD ? rest - b * p.J : rest;
   const int64_t rows = BACKWARD ? p.S : p.n * p.S;
   const int64_t r0 = j * p.chunk, r1 = r0 + p.chunk < rows ? r0 + p.chunk : rows;
-  const int g = cb * (DPK_WAVE / p.lg) + lane / p.lg, at = lane % p.lg;
+  const int across = p.lg * p.wide, side = DPK_WAVE / across, sub = lane / across;  // rows side by side, and this lane's
+  const int g = cb * p.wide + lane % across / p.lg, at = lane % p.lg;
   const bool mine = g < p.G;
   bool on[NI];
   int c[NI];
@@ -695,15 +698,16 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
       for (int i = 0; i < NI; ++i) {
         nx[q][i] = typename io::raw();
         if (BACKWARD) nd[BACKWARD ? q : 0][i] = typename io::raw();
-        if (on[i] && r + q < r1) {
-          nx[q][i] = io::load(x + (r + q) * p.C + c[i]);
-          if (BACKWARD) nd[BACKWARD ? q : 0][i] = io::load(dy + (r + q) * p.C + c[i]);
+        if (on[i] && r + q * side < r1) {
+          nx[q][i] = io::load(x + (r + q * side) * p.C + c[i]);
+          if (BACKWARD) nd[BACKWARD ? q : 0][i] = io::load(dy + (r + q * side) * p.C + c[i]);
         }
       }
     }
   };
-  fetch(r0 + wave * R);
-  for (int64_t r = r0 + wave * R; r < r1; r += kWaves * R) {
+  fetch(r0 + wave * R * side + sub);
+  // (the bound is the wave's: its lanes exchange values, so they stay together)
+  for (int64_t r = r0 + wave * R * side + sub; r - sub < r1; r += kWaves * R * side) {
     typename io::raw rx[R][NI], rd[BACKWARD ? R : 1][NI];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -713,7 +717,7 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
         if (BACKWARD) rd[BACKWARD ? q : 0][i] = nd[BACKWARD ? q : 0][i];
       }
     }
-    fetch(r + kWaves * R);  // the next rows, under this batch's arithmetic
+    fetch(r + kWaves * R * side);  // the next rows, under this batch's arithmetic
     float mean[R], rstd[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -751,7 +755,7 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
           for (int k = 0; k < V; ++k)
             z[k] = fmaf((io::get(rx[q][i], k) - mean[q]) * rstd[q], w[i * V + k], shift[i * V + k]);
           activate(z, p.act);
-          if (on[i] && r + q < r1) io::store(y + (r + q) * p.C + c[i], z);
+          if (on[i] && r + q * side < r1) io::store(y + (r + q * side) * p.C + c[i], z);
         }
       }
     } else {
@@ -771,9 +775,9 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
 #pragma unroll
           for (int k = 0; k < V; ++k) {
             // a row behind the last one has dy = 0, but its slope may not be a number times zero
-            const float dz = r + q < r1 ? io::get(rd[BACKWARD ? q : 0][i], k) * z[k] : 0.f;
+            const float dz = r + q * side < r1 ? io::get(rd[BACKWARD ? q : 0][i], k) * z[k] : 0.f;
             A[i * V + k] += dz;
-            B[i * V + k] = r + q < r1 ? fmaf(dz, xh[q][i * V + k], B[i * V + k]) : B[i * V + k];
+            B[i * V + k] = r + q * side < r1 ? fmaf(dz, xh[q][i * V + k], B[i * V + k]) : B[i * V + k];
             d[q][i * V + k] = dz * w[i * V + k];
             s1[q] += d[q][i * V + k];
             s2[q] = on[i] ? fmaf(d[q][i * V + k], xh[q][i * V + k], s2[q]) : s2[q];
@@ -791,17 +795,21 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
           float o[V];
 #pragma unroll
           for (int k = 0; k < V; ++k) o[k] = rstd[q] * (d[q][i * V + k] - s1[q] - xh[q][i * V + k] * s2[q]);
-          if (on[i] && r + q < r1) io::store(y + (r + q) * p.C + c[i], o);
+          if (on[i] && r + q * side < r1) io::store(y + (r + q * side) * p.C + c[i], o);
         }
       }
     }
   }
   if (!BACKWARD) return;
   if (!p.gw && !p.gb) return;
+  for (int o = DPK_WAVE / 2; o >= across; o /= 2) {  // the rows side by side
+#pragma unroll
+    for (int k = 0; k < N; ++k) A[k] += __shfl_xor(A[k], o, DPK_WAVE), B[k] += __shfl_xor(B[k], o, DPK_WAVE);
+  }
 #pragma unroll
   for (int k = 0; k < N; ++k) lds[0][wave][k * DPK_WAVE + lane] = A[k], lds[BACKWARD][wave][k * DPK_WAVE + lane] = B[k];
   __syncthreads();
-  if (wave != 0) return;
+  if (wave != 0 || sub != 0) return;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
 #pragma unroll
@@ -957,11 +965,14 @@ bool plan_rows(NormArgs* p, int dtype, bool backward, int* V, int* NI) {
   for (p->lg = 1; p->lg < vecs && p->lg < DPK_WAVE;) p->lg *= 2;
   for (*NI = 1; *NI * p->lg < vecs;) *NI *= 2;
   if (*NI > 4) return false;
-  p->cblocks = static_cast<int>(dpk_cdiv(p->G, DPK_WAVE / p->lg));
+  for (p->wide = 1; p->wide < p->G && p->wide * p->lg < DPK_WAVE;) p->wide *= 2;
+  p->cblocks = static_cast<int>(dpk_cdiv(p->G, p->wide));
   const int64_t rows = backward ? p->S : p->n * p->S, samples = backward ? p->n : 1;
-  // enough blocks to fill the GPU; backward, no chunk below 64 rows (the partial sums of one cost 8 bytes a channel)
+  // enough blocks to fill the GPU; backward, no chunk below 64 rows, nor 32 for every one that lies side by
+  // side in a wave (the partial sums of a chunk cost 8 bytes a channel and a reduction over the block)
   int64_t J = dpk_cdiv(kWantBlocks, samples * p->cblocks);
-  const int64_t most = dpk_cdiv(rows, backward ? 64 : 4);
+  const int64_t side = DPK_WAVE / (p->lg * p->wide);
+  const int64_t most = dpk_cdiv(rows, !backward ? 4 * side : side > 2 ? 32 * side : 64);
   if (J > most) J = most;
   if (J < 1) J = 1;
   p->chunk = dpk_cdiv(rows, J);
@@ -985,7 +996,10 @@ size_t part_bytes(int64_t n, int64_t S, int64_t C) {
   if (static_cast<size_t>(n) * J * C * sizeof(float2) > most) most = static_cast<size_t>(n) * J * C * sizeof(float2);
   return dpk_align_up(most, 256);
 }
-size_t group_bytes(int64_t n, int64_t S, int64_t G, int per_position) {
+// (mean, rstd) of every position's groups where no wave may hold one (a group of up to 256 channels fits
+// whatever its alignment), or (S1, S2) of every sample's.
+size_t group_bytes(int64_t n, int64_t S, int64_t C, int64_t G, int per_position) {
+  if (per_position && C / G <= 4 * DPK_WAVE) return 0;
   return dpk_align_up(static_cast<size_t>(n) * (per_position ? S : 1) * G * sizeof(float2), 256);
 }
 
@@ -1053,7 +1067,7 @@ void by_width(int dtype, int V, F&& body) {
 
 extern "C" size_t dpk_group_norm_act_workspace_bytes(int64_t n, int64_t S, int64_t C, int64_t groups, int per_position) {
   if (n <= 0 || S <= 0 || C <= 0 || groups <= 0) return 0;
-  return part_bytes(n, S, C) + group_bytes(n, S, groups, per_position);
+  return part_bytes(n, S, C) + group_bytes(n, S, C, groups, per_position);
 }
 
 extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, const void* bias, int param_dtype, void* y,

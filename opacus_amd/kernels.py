@@ -1081,7 +1081,7 @@ def group_norm_act(
     x = _dense(x)
     n, C = x.shape[0], x.shape[-1]
     S = math.prod(x.shape[1:-1])
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = torch.empty_like(x)
     stats = None if per_position else torch.empty((n, num_groups, 2), dtype=torch.float32, device=dev)
     if n == 0 or S == 0:
         return y, stats
@@ -1124,7 +1124,7 @@ def group_norm_act_backward(
         stats = _dense(stats)
     else:
         stats = None
-    grad_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    grad_x = torch.empty_like(x)
     if n == 0 or S == 0:
         return grad_x, torch.zeros((n, C), device=dev), torch.zeros((n, C), device=dev)
     grad_w = torch.empty((n, C), dtype=torch.float32, device=dev)

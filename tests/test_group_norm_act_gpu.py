@@ -47,7 +47,7 @@ def test_statistics_per_sample(n, S, C, groups, dtype):
 POSITION_SHAPES = [
     (1, 1, 2, 1), (3, 1, 64, 4), (2, 5, 6, 2), (2, 7, 30, 3), (1, 130, 128, 2), (4, 33, 256, 4), (2, 65, 512, 8),
     (1, 9, 1024, 16), (2, 6, 2048, 16), (2, 3, 4096, 1), (1, 4, 2048, 1), (3, 10, 100, 5), (1, 300, 40, 8), (2, 40, 96, 12),
-    (1, 2, 10000, 2), (1, 70, 8, 8), (2, 50, 24, 24),
+    (1, 2, 10000, 2), (1, 70, 8, 8), (2, 50, 24, 24), (2, 1111, 64, 2), (1, 67, 12, 3), (3, 129, 5, 5), (2, 999, 4, 1),
 ]
 
 
