@@ -5,10 +5,11 @@
 //   h_t = a_t h_{t-1} + u_t,   out_t = h_t
 //
 // The recurrence is a composition of affine maps h -> A h + B, so T is cut at will. A block takes one
-// tile of positions for 16 * V channels of a sample: every thread runs K positions of its channels in
-// registers, the block's time groups exchange their (A, B) through LDS, and the tiles of a row pass
-// the state on in one launch (see "the chain" below), so every input is read once and every output
-// written once. What is folded, and in which order, depends on sizes alone: the same bits on every run.
+// tile of positions for 32 * V channels of a sample: every thread runs K positions of its channels in
+// registers, the block's time groups exchange their (A, B) through lanes and LDS, and the tiles of a
+// row pass the state on in one launch (see "the chain" below), so every input is read once and every
+// output written once. What is folded, and in which order, depends on sizes alone: the same bits on
+// every run.
 //
 // Backward: g_t = dy_t + a_{t+1} g_{t+1} runs the same maps the other way (same A, other B), and
 //   q = 1 - a,  m = sqrt(q (1 + a)),  kappa = -L / m,  s = sigma(i)
@@ -18,6 +19,15 @@
 // this form nothing is divided by m alone, which vanishes as the gate closes.) h_{t-1} is formed
 // again from the fp32 state the forward pass kept at every 64th position, so no rounded output
 // enters a gradient.
+//
+// Bounds, at 16 x 1024 x 2048: forward bf16 54 us for 272 MB (5.0 TB/s; a large copy reaches 4.9 to 5.3), fp32 111 us
+// for 541 MB (4.9 TB/s): memory. Backward fp32 199 us for 948 MB (4.8 TB/s): memory. Backward bf16 127 us
+// for 478 MB (3.8 TB/s), 12 us of them the chain's clearing and the sum of the decay gradients: half
+// the cycles issue arithmetic (66 vector instructions an element, 6 of them transcendental), and three
+// waves a SIMD are what their registers leave to cover loads with. Tried for it and slower: 4 positions a
+// thread in blocks of 512 (four waves a SIMD, 138 us), four waves with spills (211 us), two rows a block
+// with the second one's inputs sent ahead into LDS (140 us). One 16384-token row of 2048 channels: 68 us
+// for 268 MB; a summary launch in front instead of the chain took 127 us.
 #include <initializer_list>
 
 #include "vec_io.h"
@@ -221,6 +231,16 @@ __device__ __forceinline__ void load_decay(const void* decay, int is_bf16, int64
     lam[j] = is_bf16 ? bf16_to_f32(static_cast<const bf16_t*>(decay)[c + j]) : static_cast<const float*>(decay)[c + j];
 }
 
+// The row of a block: consecutive block numbers walk the rows, so that all rows advance together.
+// Blocks go to the XCDs in turn; where a row is one 128-byte line wide (2-byte elements), each XCD gets neighbouring rows
+// instead, so that it walks through contiguous memory (16 x 1024 x 2048 bf16 backward: 128 -> 118 us; wider rows
+// do not gain: fp32 forward 110 -> 120 us, backward 200 -> 197 us).
+template <typename T>
+__device__ __forceinline__ int64_t row_of(int64_t rows) {
+  const uint32_t n = static_cast<uint32_t>(rows), i = blockIdx.x % n;
+  return sizeof(T) == 2 ? xcd_contiguous_id(i, n) : i;
+}
+
 // softplus of the decays of V channels from c on; 0 behind the last channel
 template <int V>
 __device__ __forceinline__ void softplus_of(const void* decay, int is_bf16, int64_t D, int64_t c, float (&sp)[V]) {
@@ -409,7 +429,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_ker
   __shared__ float lds_m[2 * kRun * W];
   __shared__ float lds_s[W];
   __shared__ int lds_t;
-  const int64_t cbs = (p.D + W - 1) / W, r = blockIdx.x % p.ch.rows, b = r / cbs, cb = r - b * cbs;
+  const int64_t cbs = (p.D + W - 1) / W, r = row_of<T>(p.ch.rows), b = r / cbs, cb = r - b * cbs;
   draw_tile(p.ch, r, &lds_t);
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
@@ -608,7 +628,7 @@ __global__ __launch_bounds__(kBwdThreads, 3) void scan_bwd_kernel(ScanBwdArgs p)
   __shared__ float lds_m[2 * kRun * W];
   __shared__ float lds_s[W];
   __shared__ int lds_t;
-  const int64_t cbs = (p.D + W - 1) / W, r = blockIdx.x % p.ch.rows, b = r / cbs, cb = r - b * cbs;
+  const int64_t cbs = (p.D + W - 1) / W, r = row_of<T>(p.ch.rows), b = r / cbs, cb = r - b * cbs;
   draw_tile(p.ch, r, &lds_t);
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
@@ -621,23 +641,24 @@ __global__ __launch_bounds__(kBwdThreads, 3) void scan_bwd_kernel(ScanBwdArgs p)
     bwd_tile<T, V, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_g, lds_m, lds_s);
 }
 
-// out[i] = sum over the tiles of part[tile][i]: 64 sums a block, 16 waves each on every 16th tile.
+// out[i] = sum over the tiles of part[tile][i], in order: 64 sums a block, its 16 waves on 16 neighbouring
+// runs of tiles, and those in order.
 __global__ __launch_bounds__(1024) void scan_dlam_kernel(const float* __restrict__ part, int tiles, int64_t nD,
                                                          float* __restrict__ out) {
   __shared__ float lds[16][DPK_WAVE];
-  const int lane = threadIdx.x % DPK_WAVE, wave = threadIdx.x / DPK_WAVE;
+  const int lane = threadIdx.x % DPK_WAVE, wave = threadIdx.x / DPK_WAVE, waves = blockDim.x / DPK_WAVE;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * DPK_WAVE + lane;
+  const int run = (tiles + waves - 1) / waves, k0 = wave * run, k1 = k0 + run < tiles ? k0 + run : tiles;
   float t = 0.f;
   if (i < nD) {
-#pragma unroll 4
-    for (int k = wave; k < tiles; k += 16) t += part[k * nD + i];
+#pragma unroll 8
+    for (int k = k0; k < k1; ++k) t += part[k * nD + i];
   }
   lds[wave][lane] = t;
   __syncthreads();
   if (wave == 0 && i < nD) {
     t = 0.f;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) t += lds[w][lane];
+    for (int w = 0; w < waves; ++w) t += lds[w][lane];
     out[i] = t;
   }
 }
@@ -689,8 +710,8 @@ char* chain_of(Chain* ch, int64_t n, int64_t D, int V, int tiles, void* ws, hipS
   at += dpk_align_up(static_cast<size_t>(ch->rows) * 4, 256);
   ch->maps = reinterpret_cast<uint64_t*>(at);
   ch->states = ch->maps + ch->rows * tiles * W;
-  const int64_t blocks = dpk_cdiv(words, kThreads * 4);  // two 16-byte stores a thread
-  hipLaunchKernelGGL(chain_clear_kernel, dim3(static_cast<unsigned>(blocks < 2048 ? blocks : 2048)), dim3(kThreads), 0, s,
+  const int64_t blocks = dpk_cdiv(words, kThreads * 2);  // one 16-byte store a thread
+  hipLaunchKernelGGL(chain_clear_kernel, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(kThreads), 0, s,
                      ch->tickets, ch->rows, reinterpret_cast<uint4*>(ch->maps), words / 2);
   return at + words * 8;
 }
@@ -720,8 +741,9 @@ int check_common(const char* fn, const void* gates, int dtype, const void* decay
   DPK_REQUIRE(sn >= 0 && st >= 0, DPK_E_ARG, "%s: negative stride", fn);
   DPK_REQUIRE(3 * D <= kMaxStride && (T <= 1 || st <= kMaxStride), DPK_E_SHAPE,
               "%s: a position's features span more than %lld elements", fn, (long long)kMaxStride);
-  DPK_REQUIRE(T < (1LL << 36) && n < (1LL << 31) && D < (1LL << 31) && dpk_cdiv(T + 1, kBwdTile) * dpk_cdiv(D, kCL) * n <= DPK_MAX_GRID_X,
-              DPK_E_SHAPE, "%s: n * T * D too large", fn);
+  // (in floating point: the product of sizes no tensor has must not wrap around)
+  const double blocks = static_cast<double>(n) * static_cast<double>(D / kCL + 1) * static_cast<double>(T / kBwdTile + 1);
+  DPK_REQUIRE(blocks <= static_cast<double>(DPK_MAX_GRID_X), DPK_E_SHAPE, "%s: n * T * D too large", fn);
   return DPK_OK;
 }
 
@@ -815,8 +837,8 @@ extern "C" int dpk_gated_scan_backward(const void* gates, int dtype, const void*
   }
 #undef DPK_SCAN_BWD
   if (tiles > 1 && grad_decay)
-    hipLaunchKernelGGL(scan_dlam_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * D, DPK_WAVE))), dim3(1024), 0, s, p.dlam, tiles,
-                       n * D, grad_decay);
+    hipLaunchKernelGGL(scan_dlam_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * D, DPK_WAVE))),
+                       dim3(DPK_WAVE * (tiles <= 32 ? 4 : 16)), 0, s, p.dlam, tiles, n * D, grad_decay);
   DPK_LAUNCH_CHECK(fn);
   return DPK_OK;
 }
