@@ -659,7 +659,7 @@ __device__ __forceinline__ void lane_sum(float (&v)[R], int lg) {
 }
 
 template <typename T, int V, int NI, int R, bool BACKWARD>
-__global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
+__global__ __launch_bounds__(kThreads, NI * V <= 8 ? 3 : 1) void position_rows_kernel(NormArgs p) {
   typedef vec_io<T, V> io;
   constexpr int N = NI * V, kWaves = kThreads / DPK_WAVE;
   __shared__ float lds[BACKWARD ? 2 : 1][BACKWARD ? kWaves : 1][BACKWARD ? DPK_WAVE * N : 1];
@@ -736,22 +736,26 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
       }
     }
     lane_sum(mean, p.lg);
+    // A lane without a channel takes 0 for the mean, a row behind the last one 0 for rstd: their x and dy
+    // are zeros, so every term they add is zero too and no element has to be masked.
+    float at_mean[R][NI];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       mean[q] *= inv;
       rstd[q] = 0.f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
+        at_mean[q][i] = on[i] ? mean[q] : 0.f;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float d = io::get(rx[q][i], k) - mean[q];
-          rstd[q] = on[i] ? fmaf(d, d, rstd[q]) : rstd[q];
+          const float d = io::get(rx[q][i], k) - at_mean[q][i];
+          rstd[q] = fmaf(d, d, rstd[q]);
         }
       }
     }
     lane_sum(rstd, p.lg);
 #pragma unroll
-    for (int q = 0; q < R; ++q) rstd[q] = 1.0f / sqrtf(fmaf(rstd[q], inv, p.eps));
+    for (int q = 0; q < R; ++q) rstd[q] = r + q * side < r1 ? 1.0f / sqrtf(fmaf(rstd[q], inv, p.eps)) : 0.f;
     if (!BACKWARD) {
 #pragma unroll
       for (int q = 0; q < R; ++q) {
@@ -760,7 +764,7 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
           float z[V];
 #pragma unroll
           for (int k = 0; k < V; ++k)
-            z[k] = fmaf((io::get(rx[q][i], k) - mean[q]) * rstd[q], w[i * V + k], shift[i * V + k]);
+            z[k] = fmaf((io::get(rx[q][i], k) - at_mean[q][i]) * rstd[q], w[i * V + k], shift[i * V + k]);
           activate(z, p.act);
           if (on[i] && r + q * side < r1) io::store(y + (r + q * side) * p.C + c[i], z);
         }
@@ -775,19 +779,18 @@ __global__ __launch_bounds__(kThreads) void position_rows_kernel(NormArgs p) {
           float z[V];
 #pragma unroll
           for (int k = 0; k < V; ++k) {
-            xh[q][i * V + k] = (io::get(rx[q][i], k) - mean[q]) * rstd[q];
+            xh[q][i * V + k] = (io::get(rx[q][i], k) - at_mean[q][i]) * rstd[q];
             z[k] = fmaf(xh[q][i * V + k], w[i * V + k], shift[i * V + k]);
           }
           slope(z, p.act);
 #pragma unroll
           for (int k = 0; k < V; ++k) {
-            // a row behind the last one has dy = 0, but its slope may not be a number times zero
-            const float dz = r + q * side < r1 ? io::get(rd[BACKWARD ? q : 0][i], k) * z[k] : 0.f;
+            const float dz = io::get(rd[BACKWARD ? q : 0][i], k) * z[k];
             A[i * V + k] += dz;
-            B[i * V + k] = r + q * side < r1 ? fmaf(dz, xh[q][i * V + k], B[i * V + k]) : B[i * V + k];
+            B[i * V + k] = fmaf(dz, xh[q][i * V + k], B[i * V + k]);
             d[q][i * V + k] = dz * w[i * V + k];
             s1[q] += d[q][i * V + k];
-            s2[q] = on[i] ? fmaf(d[q][i * V + k], xh[q][i * V + k], s2[q]) : s2[q];
+            s2[q] = fmaf(d[q][i * V + k], xh[q][i * V + k], s2[q]);
           }
         }
       }
