@@ -20,14 +20,15 @@
 // again from the fp32 state the forward pass kept at every 64th position, so no rounded output
 // enters a gradient.
 //
-// Bounds, at 16 x 1024 x 2048: forward bf16 54 us for 272 MB (5.0 TB/s; a large copy reaches 4.9 to 5.3), fp32 111 us
-// for 541 MB (4.9 TB/s): memory. Backward fp32 199 us for 948 MB (4.8 TB/s): memory. Backward bf16 127 us
-// for 478 MB (3.8 TB/s), 12 us of them the chain's clearing and the sum of the decay gradients: half
-// the cycles issue arithmetic (66 vector instructions an element, 6 of them transcendental), and three
-// waves a SIMD are what their registers leave to cover loads with. Tried for it and slower: 4 positions a
-// thread in blocks of 512 (four waves a SIMD, 138 us), four waves with spills (211 us), two rows a block
-// with the second one's inputs sent ahead into LDS (140 us). One 16384-token row of 2048 channels: 68 us
-// for 268 MB; a summary launch in front instead of the chain took 127 us.
+// Bounds, at 16 x 1024 x 2048: forward bf16 54 us for 272 MB (5.0 TB/s; a large copy reaches 4.9 to 5.3), fp32 110 us
+// for 541 MB (4.9 TB/s): memory. Backward fp32 200 us for 948 MB (4.7 TB/s): memory. Backward bf16 118 us for 478 MB
+// (4.1 TB/s), about 10 us of them the chain's clearing and the sum of the decay gradients: half the
+// cycles issue arithmetic (62 vector instructions an element, 6 of them transcendental), and three waves
+// a SIMD are what their registers leave to cover loads with. Tried for it and slower: 4 positions a thread
+// in blocks of 512 (four waves a SIMD, 130 us), two waves with nothing spilled (134 us), four with spills
+// (211 us against 126 then), two rows a block with the second one's inputs sent ahead into LDS (140 us
+// against 126 then). One 16384-token row of 2048 channels: 68 us for 268 MB; a summary launch in front
+// instead of the chain took 127 us.
 #include <initializer_list>
 
 #include "vec_io.h"

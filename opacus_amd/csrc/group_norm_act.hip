@@ -15,11 +15,10 @@
 // holds, and put together from (count, mean, M2) triples, so that a large mean costs no digits.
 // All arithmetic is fp32; every reduction runs in a fixed order.
 //
-// Memory bounds all of it but the erf form of gelu (about 23 instructions a value, so that the two
-// backward passes over 3 x 40000 x 128 bf16 issue arithmetic three quarters of their time). Training passes
-// (forward and backward): 256 x 1024 x 64 fp32, 32 groups: 67 us for 336 MB (5.0 TB/s); per position 16 x 1024 x 2048
-// bf16, 16 heads: 78 us for 335 MB (4.3 TB/s; the forward pass alone 28 us, 4.8 TB/s); 3 x 40000 x 128 bf16, 32 groups, gelu:
-// 80 us for 215 MB in six launches.
+// Training passes (forward and backward): 256 x 1024 x 64 fp32, 32 groups: 67 us for 336 MB (5.0 TB/s), memory; per
+// position 16 x 1024 x 2048 bf16, 16 heads: 72 us for 335 MB (4.6 TB/s), memory and, backward, arithmetic (three
+// quarters of the issue slots); 3 x 40000 x 128 bf16, 32 groups, gelu: 80 us for 215 MB in six launches, half of the
+// issue slots arithmetic (gelu takes about 23 instructions a value in each of three passes), 10 us merges.
 #include <type_traits>
 
 #include "vec_io.h"
