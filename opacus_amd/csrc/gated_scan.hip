@@ -112,23 +112,27 @@ __device__ __forceinline__ void publish(uint64_t* w, float a, float b) {
   const uint32_t lo = a != a ? 0x7fc00000u : __float_as_uint(a);
   __hip_atomic_store(w, (static_cast<uint64_t>(__float_as_uint(b)) << 32) | lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// Waits until all V words are written. A block waits microseconds; what would keep it for 2^21 reads (seconds
+// of running) is a workspace that another call wrote to meanwhile, against the rules of the C interface. The
+// wait then ends with NaN for the state, so that even such a launch drains.
+constexpr uint32_t kMostReads = 1u << 21;
 template <int V>
 __device__ __forceinline__ void await(const uint64_t* w, float* a, float* b) {
   uint64_t v[V];
-  bool there;
-  do {
+  bool there = false;
+  for (uint32_t reads = 0; !there && reads < kMostReads; ++reads) {
+    if (reads) __builtin_amdgcn_s_sleep(1);
     there = true;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       v[j] = __hip_atomic_load(w + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       there = there && static_cast<uint32_t>(v[j]) != kEmpty;
     }
-    if (!there) __builtin_amdgcn_s_sleep(1);
-  } while (!there);
+  }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    a[j] = __uint_as_float(static_cast<uint32_t>(v[j]));
-    b[j] = __uint_as_float(static_cast<uint32_t>(v[j] >> 32));
+    a[j] = there ? __uint_as_float(static_cast<uint32_t>(v[j])) : __uint_as_float(0x7fc00000u);
+    b[j] = there ? __uint_as_float(static_cast<uint32_t>(v[j] >> 32)) : __uint_as_float(0x7fc00000u);
   }
 }
 
@@ -435,6 +439,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_ker
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
   const int t = drawn_tile(&lds_t);
+  if (t >= p.ch.tiles) return;  // never, unless another call used the workspace meanwhile
   const Tile tl = tile_of<TILE>(p.T, live_length(p.lengths, b, p.T), static_cast<int64_t>(t) * TILE, p.reverse);
   if (tl.hi - tl.lo == TILE && (cb + 1) * W <= p.D) fwd_tile<T, V, K, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
   else fwd_tile<T, V, K, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
@@ -634,6 +639,7 @@ __global__ __launch_bounds__(kBwdThreads, 3) void scan_bwd_kernel(ScanBwdArgs p)
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
   const int t = drawn_tile(&lds_t);  // 0 is the last tile of the scan
+  if (t >= p.ch.tiles) return;  // never, unless another call used the workspace meanwhile
   const Tile tl = tile_of<kBwdTile>(p.T, live_length(p.lengths, b, p.T),
                                     static_cast<int64_t>(p.ch.tiles - 1 - t) * kBwdTile, p.reverse);
   if (tl.hi - tl.lo == kBwdTile && (cb + 1) * W <= p.D)

@@ -295,3 +295,83 @@ def test_another_stream():
         got = kernels.gated_scan(gates, decay, state, lengths)
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(p, q) for p, q in zip(got[:2], want[:2]))
+
+
+def test_graphs_that_share_a_memory_pool_replay_in_turn():
+    """The second graph's workspaces lie where the first one's were."""
+    from opacus_amd import kernels
+
+    a, b = make(1, 1500, 64, torch.bfloat16, seed=21, with_state=True), make(2, 900, 40, torch.float32, seed=22, with_state=True)
+
+    def call(t):
+        gates, decay, state, _, dy, dl = t
+        out, last, kept = kernels.gated_scan(gates, decay, state, keep_states=True)
+        return (out, last) + kernels.gated_scan_backward(gates, decay, kept, dy, dl)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(a), call(b)
+    torch.cuda.current_stream().wait_stream(side)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        ra = call(a)
+    with torch.cuda.graph(second, pool=first.pool()):
+        rb = call(b)
+    want_a, want_b = call(a), call(b)
+    for _ in range(3):
+        first.replay()
+        second.replay()
+        call(b)
+        torch.cuda.synchronize()
+        for p, q in zip(ra + rb, want_a + want_b):
+            assert torch.equal(p, q)
+
+
+def test_two_calls_on_two_streams_at_once():
+    from opacus_amd import kernels
+
+    sets = [make(4, 3000, 128, torch.bfloat16, seed=30 + k) for k in range(2)]
+    want = [kernels.gated_scan(g, d, keep_states=True) for g, d, *_ in sets]
+    want_b = [kernels.gated_scan_backward(s[0], s[1], w[2], s[4]) for s, w in zip(sets, want)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                out = kernels.gated_scan(sets[k][0], sets[k][1], keep_states=True)
+                got[k].append(out + kernels.gated_scan_backward(sets[k][0], sets[k][1], out[2], sets[k][4]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for res in got[k]:
+            for p, q in zip(res, want[k] + want_b[k]):
+                assert torch.equal(p, q)
+
+
+def test_offsets_past_32_bits():
+    """3.2 billion gate elements: the second sample's results against the same sample alone, whose
+    offsets are small. What is folded, and how, depends on T and D alone: the same bits."""
+    from opacus_amd import kernels
+
+    n, T, D = 2, 65536, 8192
+    g = torch.Generator(device="cuda").manual_seed(5)
+    gates = torch.empty(n, T, 3 * D, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    assert gates.numel() > 2**31
+    dy = torch.empty(n, T, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    decay = torch.randn(D, device="cuda", generator=g)
+    out, last, kept = kernels.gated_scan(gates, decay, keep_states=True)
+    dg, dd, ds = kernels.gated_scan_backward(gates, decay, kept, dy)
+    one, one_dy = gates[1:].clone(), dy[1:].clone()
+    out1, last1, kept1 = kernels.gated_scan(one, decay, keep_states=True)
+    dg1, dd1, ds1 = kernels.gated_scan_backward(one, decay, kept1, one_dy)
+    for p, q in ((out, out1), (last, last1), (kept, kept1), (dg, dg1), (dd, dd1), (ds, ds1)):
+        assert torch.equal(p[1:], q)
+    # and a slice of it against the definition: the first 40 positions of the last 8 channels
+    from _scan_reference import assert_within, scan_reference
+
+    cols = torch.cat([torch.arange(k * D + D - 8, k * D + D, device="cuda") for k in range(3)])
+    sub = gates[1:, :40].index_select(2, cols)
+    val, tol = scan_reference(sub.clamp(-8, 8), decay[-8:])
+    assert_within(out[1:, :40, -8:], val["out"], tol["out"], "out")

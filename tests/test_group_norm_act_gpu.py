@@ -196,3 +196,34 @@ def test_captured_calls_replay_on_new_inputs(S, C, groups, per_position):
         for _, res in graphs:
             for p, q in zip(res, want):
                 assert torch.equal(p, q)
+
+
+def test_offsets_past_32_bits():
+    """2.2 billion elements: the last rows against the same rows in a small tensor."""
+    from opacus_amd import kernels
+
+    S, C, G = 17_000_000, 64, 4
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.empty(2, S, C, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    dy = torch.empty(2, S, C, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    assert x.numel() > 2**31
+    w, b = torch.rand(C, device="cuda", generator=g) + 0.5, torch.randn(C, device="cuda", generator=g)
+    args = (G, w, b, 1e-5, "silu")
+    y, _ = kernels.group_norm_act(x, *args, per_position=True)
+    dx, dw, db = kernels.group_norm_act_backward(x, dy, None, *args, per_position=True)
+    xs, dys = x[1:, -50:].clone(), dy[1:, -50:].clone()
+    ys, _ = kernels.group_norm_act(xs, *args, per_position=True)
+    dxs, _, _ = kernels.group_norm_act_backward(xs, dys, None, *args, per_position=True)
+    assert torch.equal(y[1:, -50:], ys) and torch.equal(dx[1:, -50:], dxs)
+    # per sample: the second sample alone is cut into other chunks, so sums agree to their rounding
+    y, st = kernels.group_norm_act(x, *args)
+    dx, dw, db = kernels.group_norm_act_backward(x, dy, st, *args)
+    one, one_dy = x[1:].clone(), dy[1:].clone()
+    y1, st1 = kernels.group_norm_act(one, *args)
+    dx1, dw1, db1 = kernels.group_norm_act_backward(one, one_dy, st1, *args)
+    # 264 half-steps of the sums' terms: mean |x| is 0.8, the variance 1, mean |dz| below 1, and sums of S terms
+    bar = 264 * 2.0**-24
+    assert (st[1] - st1[0]).abs().max() <= 2 * bar
+    assert (dw[1] - dw1[0]).abs().max() <= 2 * bar * S and (db[1] - db1[0]).abs().max() <= 2 * bar * S
+    # outputs: at most a rounding apart (2**-8 of values below 16 and of gradients below 16)
+    assert (y[1] - y1[0]).abs().max() <= 2.0**-4 and (dx[1] - dx1[0]).abs().max() <= 2.0**-4
