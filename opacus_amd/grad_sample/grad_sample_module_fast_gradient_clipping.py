@@ -394,7 +394,9 @@ class GradSampleHooksFastGradientClipping(GradSampleHooks):
                 small = sum(gs.numel() for gs in grad_samples.values()) <= self.KEEP_GRAD_SAMPLES_BELOW
                 # (copies: a tensor adopted as p._current_grad_sample has later uses of the module added into it)
                 kept_gs = {p: gs.clone() for p, gs in grad_samples.items()} if small else None
-                self._kept_passes.append((module, activations, backprops, scale, kept_gs))
+                # the samplers of per-sample rows read backprops alone: the layer's inputs may go
+                acts = [] if getattr(module, "per_sample_rows", False) else activations
+                self._kept_passes.append((module, acts, backprops, scale, kept_gs))
             adopt = getattr(sampler, "owns_output", False)
             for param, gs in grad_samples.items():
                 create_or_accumulate_grad_sample(

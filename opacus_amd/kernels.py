@@ -1036,7 +1036,8 @@ def gated_scan_step(gates: torch.Tensor, decay: torch.Tensor, state: torch.Tenso
         _at(gates), _code(gates), _at(decay), _code(decay), _at(state), _at(out), n, D,
         gates.stride(0) if n > 1 else 3 * D,
     )
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():  # (tensors made in inference mode have no version to count)
+        torch.autograd.graph.increment_version(state)
     return out
 
 

@@ -365,3 +365,57 @@ def test_a_captured_training_pass_replays():
         torch.cuda.synchronize()
         for p, q in zip(got, want):
             assert_rel(p.reshape(1, -1), q.reshape(1, -1), 1e-5, f"replay {k}")
+
+
+def test_inference_mode_and_kernel_times():
+    from opacus_amd import kernels
+    from opacus_amd.layers import DPGatedRNN
+
+    torch.manual_seed(11)
+    rnn = DPGatedRNN(6, 24, 2, batch_first=True, num_heads=4).cuda()
+    x = torch.randn(3, 9, 6, device="cuda")
+    want, last = rnn(x)
+    with torch.inference_mode(), kernels.record_kernel_times() as times:
+        out, h = rnn(x[:, :8])
+        y = rnn.step(x[:, 8], h)
+        state = rnn.initial_state(3)
+        for t in range(9):
+            z = rnn.step(x[:, t], state)
+    torch.cuda.synchronize()
+    assert set(times) == {"gated_scan", "gated_scan_step", "group_norm_act"}
+    assert all(s.elapsed_time(e) >= 0 for pairs in times.values() for s, e in pairs)
+    for got in (y, z):
+        assert_rel(got, want[:, -1], 1e-4, "output")
+    assert_rel(state, last, 1e-4, "state")
+
+
+def test_large_rows_take_the_clipped_sum_from_the_rows_again():
+    """Per-sample gradients too large to be kept (KEEP_GRAD_SAMPLES_BELOW) are taken from the rows a second time."""
+    from opacus_amd import GradSampleModuleFastGradientClipping
+    from opacus_amd.layers import HeadNormAct
+    from opacus_amd.optimizers import DPOptimizerFastGradientClipping
+    from opacus_amd.utils.fast_gradient_clipping_utils import DPLossFastGradientClipping
+
+    class Loss(nn.Module):
+        reduction = "sum"
+
+        def forward(self, out, tgt):
+            l = (out - tgt).pow(2).flatten(1).sum(1)
+            return l if self.reduction == "none" else l.sum()
+
+    torch.manual_seed(12)
+    grads = []
+    for keep in (1 << 22, 0):
+        torch.manual_seed(13)
+        norm = HeadNormAct(4, 32).cuda()
+        model = GradSampleModuleFastGradientClipping(norm, loss_reduction="sum", max_grad_norm=0.5)
+        model.KEEP_GRAD_SAMPLES_BELOW = keep
+        opt = DPOptimizerFastGradientClipping(
+            torch.optim.SGD(norm.parameters(), lr=0.1), noise_multiplier=0.0, max_grad_norm=0.5, expected_batch_size=5,
+            loss_reduction="sum",
+        )
+        x, t = torch.randn(5, 7, 32, device="cuda"), torch.randn(5, 7, 32, device="cuda")
+        DPLossFastGradientClipping(model, opt, Loss(), loss_reduction="sum")(model(x), t).backward()
+        grads.append([p.grad.clone() for p in norm.parameters()])
+    for p, q in zip(*grads):
+        assert torch.equal(p, q) and p.abs().max() > 0
