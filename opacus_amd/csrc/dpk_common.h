@@ -38,6 +38,8 @@ static inline size_t dpk_align_up(size_t x, size_t a) { return (x + a - 1) / a *
 // Grid dimension limits of HIP: x up to 2^31-1, y and z up to 65535.
 #define DPK_MAX_GRID_X 2147483647LL
 #define DPK_MAX_GRID_YZ 65535LL
+// and fewer than 2^32 threads along x.
+static inline bool dpk_grid_fits(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
 
 // ---- device side -----------------------------------------------------------
 #if defined(__HIPCC__)

@@ -89,7 +89,7 @@ __device__ __forceinline__ float inv_scale(float q2) { return __builtin_amdgcn_r
 
 // ---- the chain: tiles of one row hand the state on within a launch -----------------------------
 //
-// A row is 16 * V channels of one sample; its tiles are numbered by a ticket each block draws when
+// A row is 32 * V channels of one sample; its tiles are numbered by a ticket each block draws when
 // it starts, so a block only ever waits for blocks that are already running and that never wait
 // for it. Every tile but the row's last publishes its (A, B); 16 tiles form a run, and the last
 // tile of a run publishes the state after it. A tile waits for the (A, B) of the tiles before it in its
@@ -699,7 +699,7 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(const T* __restrict
 
 int tiles_of(int64_t T, int tile) { return T > tile ? static_cast<int>(dpk_cdiv(T, tile)) : 1; }
 
-// The chain's part of the workspace for rows of 16 * V channels: tickets, maps, states.
+// The chain's part of the workspace for rows of 32 * V channels: tickets, maps, states.
 size_t chain_bytes(int64_t n, int64_t D, int V, int tiles) {
   if (tiles == 1) return 0;
   const size_t rows = static_cast<size_t>(n * dpk_cdiv(D, kCL * V));
@@ -781,6 +781,7 @@ extern "C" int dpk_gated_scan(const void* gates, int dtype, const void* decay, i
               DPK_E_ALIGN, "%s: a tensor is not aligned to its element size", fn);
   const int V = vec_of(2, D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, out}, {last, state, kept});
   const int tiles = tiles_of(T, kFwdTile);
+  DPK_REQUIRE(dpk_grid_fits(n * dpk_cdiv(D, kCL * V) * tiles, kThreads), DPK_E_SHAPE, "%s: n * T * D too large", fn);
   const size_t need = chain_bytes(n, D, V, tiles);
   DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
   DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
@@ -825,6 +826,7 @@ extern "C" int dpk_gated_scan_backward(const void* gates, int dtype, const void*
   const int V = vec_of(2, D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, grad_out, grad_gates},
                        {kept, grad_last, grad_decay, grad_state});
   const int tiles = tiles_of(T, kBwdTile);
+  DPK_REQUIRE(dpk_grid_fits(n * dpk_cdiv(D, kCL * V) * tiles, kBwdThreads), DPK_E_SHAPE, "%s: n * T * D too large", fn);
   const size_t need = chain_bytes(n, D, V, tiles) + (tiles > 1 && grad_decay ? static_cast<size_t>(tiles) * n * D * 4 : 0);
   DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
   DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
@@ -859,6 +861,7 @@ extern "C" int dpk_gated_scan_step(const void* gates, int dtype, const void* dec
   DPK_REQUIRE(dpk_aligned(out, dpk_elsize(dtype)) && dpk_aligned(state, 4), DPK_E_ALIGN,
               "%s: a tensor is not aligned to its element size", fn);
   const int V = vec_of(4, D, dtype, gates_stride_n, 0, n, 1, {gates, out}, {state});
+  DPK_REQUIRE(dpk_grid_fits(dpk_cdiv(n * (D / V), kThreads), kThreads), DPK_E_SHAPE, "%s: n * D too large", fn);
   const unsigned grid = static_cast<unsigned>(dpk_cdiv(n * (D / V), kThreads));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int db = decay_dtype == DPK_BF16;

@@ -558,9 +558,8 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(NormArgs p) {
       }
     }
     slab_sums<V>(t, on, rg, lane, step, W, p.Cg, lds, chan[0], grp[1], nullptr);
-    if (threadIdx.x < gs)
-      for (int g = threadIdx.x; g < gs; g += kSlabThreads)
-        p.stats[b * p.G + g0 + g] = make_float2(grp[0][g] * inv, 1.0f / sqrtf(fmaf(grp[1][g], inv, p.eps)));
+    for (int g = threadIdx.x; g < gs; g += kSlabThreads)
+      p.stats[b * p.G + g0 + g] = make_float2(grp[0][g] * inv, 1.0f / sqrtf(fmaf(grp[1][g], inv, p.eps)));
 #pragma unroll
     for (int j = 0; j < V; ++j) rstd[j] = w[j] / sqrtf(fmaf(grp[1][(in + j) / p.Cg], inv, p.eps));
 #pragma unroll
@@ -933,7 +932,7 @@ void plan(NormArgs* p, int V, bool sums) {
 
 int grid_of(const char* fn, const NormArgs& p, dim3* grid) {
   const int64_t blocks = p.n * p.cblocks * p.J;
-  DPK_REQUIRE(blocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+  DPK_REQUIRE(dpk_grid_fits(blocks, kThreads), DPK_E_SHAPE, "%s: too large", fn);
   *grid = dim3(static_cast<unsigned>(blocks));
   return DPK_OK;
 }
@@ -1095,9 +1094,10 @@ extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, 
   hipStream_t s = static_cast<hipStream_t>(stream);
   int V, NI;
   if (per_position && plan_rows(&p, dtype, false, &V, &NI)) {
-    DPK_REQUIRE(static_cast<int64_t>(p.J) * p.cblocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+    DPK_REQUIRE(dpk_grid_fits(static_cast<int64_t>(p.J) * p.cblocks, kThreads), DPK_E_SHAPE, "%s: too large", fn);
     by_width(dtype, V, [&](auto t, auto v) { launch_rows<decltype(t), decltype(v)::value, false>(p, NI, s); });
   } else if (per_position) {
+    DPK_REQUIRE(dpk_grid_fits(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE), kThreads), DPK_E_SHAPE, "%s: too large", fn);
     const unsigned grid = static_cast<unsigned>(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE));
     if (dtype == DPK_BF16) hipLaunchKernelGGL((position_kernel<bf16_t, false>), dim3(grid), dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL((position_kernel<float, false>), dim3(grid), dim3(kThreads), 0, s, p);
@@ -1105,10 +1105,12 @@ extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, 
     V = width_of(p, dtype);
     int R;
     if (plan_slabs(&p, V, dtype, &R)) {
+      DPK_REQUIRE(dpk_grid_fits(n * p.cblocks, kSlabThreads), DPK_E_SHAPE, "%s: too large", fn);
       by_width(dtype, V, [&](auto t, auto v) { launch_slabs<decltype(t), decltype(v)::value, false>(p, R, s); });
       DPK_LAUNCH_CHECK(fn);
       return DPK_OK;
     }
+    DPK_REQUIRE(dpk_grid_fits(n * groups, kThreads), DPK_E_SHAPE, "%s: too many groups", fn);
     plan(&p, V, true);
     p.part = static_cast<float2*>(ws);
     dim3 grid;
@@ -1148,7 +1150,7 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
   p.part = static_cast<float2*>(ws);
   int V, NI;
   if (per_position && plan_rows(&p, dtype, true, &V, &NI)) {
-    DPK_REQUIRE(n * p.J * p.cblocks <= DPK_MAX_GRID_X, DPK_E_SHAPE, "%s: too large", fn);
+    DPK_REQUIRE(dpk_grid_fits(n * p.J * p.cblocks, kThreads), DPK_E_SHAPE, "%s: too large", fn);
     by_width(dtype, V, [&](auto t, auto v) { launch_rows<decltype(t), decltype(v)::value, true>(p, NI, s); });
     if (p.J > 1 && (p.gw || p.gb))
       hipLaunchKernelGGL(chunk_merge_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * C, kThreads))), dim3(kThreads), 0, s, p);
@@ -1158,6 +1160,7 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
   V = width_of(p, dtype);
   int R;
   if (!per_position && plan_slabs(&p, V, dtype, &R)) {
+    DPK_REQUIRE(dpk_grid_fits(n * p.cblocks, kSlabThreads), DPK_E_SHAPE, "%s: too large", fn);
     by_width(dtype, V, [&](auto t, auto v) { launch_slabs<decltype(t), decltype(v)::value, true>(p, R, s); });
     DPK_LAUNCH_CHECK(fn);
     return DPK_OK;
@@ -1167,6 +1170,7 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
   if (int rc = grid_of(fn, p, &grid)) return rc;
   float2* groups_ws = reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(n, S, C));
   if (per_position) {
+    DPK_REQUIRE(dpk_grid_fits(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE), kThreads), DPK_E_SHAPE, "%s: too large", fn);
     p.stats = groups_ws;
     const unsigned waves = static_cast<unsigned>(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE));
     if (dtype == DPK_BF16) hipLaunchKernelGGL((position_kernel<bf16_t, true>), dim3(waves), dim3(kThreads), 0, s, p);
@@ -1178,6 +1182,7 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
       hipLaunchKernelGGL(chunk_merge_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * C, kThreads))), dim3(kThreads), 0, s, p);
     }
   } else {
+    DPK_REQUIRE(dpk_grid_fits(n * groups, kThreads), DPK_E_SHAPE, "%s: too many groups", fn);
     p.sums = groups_ws;
     by_width(dtype, V, [&](auto t, auto v) {
       hipLaunchKernelGGL((channel_sums_kernel<decltype(t), decltype(v)::value, false>), grid, dim3(kThreads), 0, s, p);

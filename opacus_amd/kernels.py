@@ -1127,7 +1127,7 @@ def group_norm_act_backward(
         stats = None
     grad_x = torch.empty_like(x)
     if n == 0 or S == 0:
-        return grad_x, torch.zeros((n, C), device=dev), torch.zeros((n, C), device=dev)
+        return grad_x, *(torch.zeros((n, C), dtype=torch.float32, device=dev) for _ in range(2))
     grad_w = torch.empty((n, C), dtype=torch.float32, device=dev)
     grad_b = torch.empty((n, C), dtype=torch.float32, device=dev)
     L = lib()

@@ -85,6 +85,20 @@ def test_c_entry_points_refuse_before_any_launch():
     assert step(None, 0, None, 0, None, None, 0, 8, 24, None) == 0
 
 
+def test_more_threads_than_a_launch_may_have_are_refused():
+    from opacus_amd import _lib
+
+    L = _lib.lib()
+    one, SHAPE = 4096, -1
+    # a block of 256 threads takes a tile of a sample: 2^24 samples are 2^32 threads
+    n = 2**24
+    assert L.dpk_gated_scan(one, 0, one, 0, None, None, one, one, None, n, 1, 1, 3, 3, 0, None, 0, None) == SHAPE
+    assert L.dpk_gated_scan_backward(
+        one, 0, one, 0, one, None, one, None, one, None, None, n, 1, 1, 3, 3, 0, None, 0, None
+    ) == SHAPE
+    assert L.dpk_gated_scan_step(one, 0, one, 0, one, one, 2**30, 31, 93, None) == SHAPE
+
+
 def test_wrappers_take_gpu_tensors_only():
     from opacus_amd import kernels
 

@@ -64,6 +64,29 @@ def test_c_entry_points_refuse_before_any_launch():
     assert L.dpk_group_norm_act_workspace_bytes(0, 4, 8, 2, 0) == 0
 
 
+@pytest.mark.parametrize(
+    "n, S, C, groups, per_position",
+    [
+        (2**23, 1, 8, 2, 0),  # a block of 512 threads per sample
+        (2**24, 2**20, 8, 2, 0),  # at least one block of 256 per chunk of a sample
+        (2**24, 1, 8, 2, 1),  # and backward, per position (forward cuts all positions of the tensor together)
+        (2**24, 16, 2**20, 1, 1),  # a wave per position
+    ],
+)
+def test_more_threads_than_a_launch_may_have_are_refused(n, S, C, groups, per_position):
+    from opacus_amd import _lib
+
+    L = _lib.lib()
+    one, big, SHAPE = 4096, 1 << 62, -1
+    if (C, per_position) != (8, 1):
+        assert L.dpk_group_norm_act(
+            one, 0, one, one, 0, one, one, n, S, C, groups, 1e-5, 0, per_position, one, big, None
+        ) == SHAPE
+    assert L.dpk_group_norm_act_backward(
+        one, one, 0, one, one, 0, one, one, one, one, n, S, C, groups, 1e-5, 0, per_position, one, big, None
+    ) == SHAPE
+
+
 def test_wrappers_refuse():
     from opacus_amd import kernels
 
