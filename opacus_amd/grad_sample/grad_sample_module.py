@@ -32,6 +32,7 @@ from ..utils.module_utils import (
     trainable_parameters,
 )
 from .. import kernels
+from ..layers.param_rows import rows_dim
 from ._common import tag_sumsq
 from .lazy import LazyLinearGradSample, lazy_linear_grad_sample
 from .functorch import ft_compute_per_sample_gradient, prepare_layer
@@ -259,7 +260,8 @@ class GradSampleHooks(AbstractGradSampleHooks):
         self.autograd_grad_sample_hooks = self._module.autograd_grad_sample_hooks
         for module in self.iterate_submodules(self._module):
             if getattr(module, "per_sample_rows", False):
-                module.__dict__["_dpk_rows_hooked"] = True
+                follows = getattr(module, "follows_layout", False)
+                module.__dict__["_dpk_rows_hooked"] = 0 if batch_first or not follows else 1
             if force_functorch or self._get_module_type(module) not in self.GRAD_SAMPLERS:
                 prepare_layer(module, batch_first=batch_first)
             elif not self.autograd_weight_grads:
@@ -477,8 +479,10 @@ class GradSampleHooks(AbstractGradSampleHooks):
             raise ValueError(f"No activations detected for {type(module)}, run forward after add_hooks(model)")
         # the recurrent layers feed their RNNLinear batch first whatever the model's layout
         # (grad_sample_module.py:391)
-        always_first = getattr(module, "stack_uses", False) or getattr(module, "per_sample_rows", False)
-        batch_dim = 0 if batch_first or always_first else 1
+        rows = getattr(module, "per_sample_rows", False)
+        batch_dim = 0 if batch_first or getattr(module, "stack_uses", False) else 1
+        if rows:
+            batch_dim = rows_dim(module)
         if "max_batch_len" not in module.__dict__:
             module.__dict__["max_batch_len"] = _get_batch_size(module=module, batch_dim=batch_dim)
         activations = module.activations.pop()
@@ -488,7 +492,7 @@ class GradSampleHooks(AbstractGradSampleHooks):
             scale = 1.0
         else:
             raise ValueError(f"loss_reduction = {loss_reduction}. Only 'sum' and 'mean' losses are supported")
-        if batch_dim != 0:
+        if batch_dim != 0 and not rows:  # (the parameters' rows are samples first)
             activations = [_batch_first_view(t, batch_dim) for t in activations]
             backprops = _batch_first_view(backprops, batch_dim)
         return activations, backprops, scale

@@ -106,6 +106,8 @@ class DPGatedRNNCell(nn.Module):
             nn.init.uniform_(p, -stdv, stdv)
         self.scan = GatedScan(hidden_size, reverse)
         self.norm = None if num_heads is None else HeadNormAct(num_heads, hidden_size, activation="silu")
+        if self.norm is not None:
+            self.norm.follows_layout = False  # fed batch first whatever the model's layout
 
     def forward(self, x: Tensor, state: Optional[Tensor], lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
         out, last = self.scan(self.ih(x), state, lengths)

@@ -15,7 +15,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .. import _lib, kernels
-from .param_rows import first_derivative_only, parameter_rows
+from .param_rows import first_derivative_only, parameter_rows, rows_dim
 
 
 class _NormActFn(torch.autograd.Function):
@@ -43,8 +43,7 @@ class _NormActFn(torch.autograd.Function):
 
 
 class _NormAct(nn.Module):
-    # the grad-sample hooks listen to the parameters' per-sample rows, which are batch first
-    # whatever the model's layout
+    # the grad-sample hooks listen to the parameters' per-sample rows
     per_sample_rows = True
     per_position: bool
 
@@ -114,11 +113,17 @@ class HeadNormAct(_NormAct):
     """``activation`` of the group norm of every position on its own: ``[n, *, C]`` with the channels
     last, ``num_groups`` heads of ``C / num_groups`` neighbouring channels, statistics over one head
     of one position. The norm of the heads of an attention or recurrence output; causal, since no
-    position sees another."""
+    position sees another. In a model wrapped with ``batch_first=False`` the samples lie along the
+    second dimension, as they do for ``nn.LayerNorm`` there."""
 
     per_position = True
+    follows_layout = True
 
     def forward(self, x: Tensor) -> Tensor:
         if x.dim() < 2:
             raise ValueError(f"expected [n, *, C], got {tuple(x.shape)}")
-        return self._apply_to(x)
+        if rows_dim(self) == 0:
+            return self._apply_to(x)
+        if x.dim() < 3:
+            raise ValueError(f"expected [T, n, *, C] in a model with batch_first=False, got {tuple(x.shape)}")
+        return self._apply_to(x.transpose(0, 1)).transpose(0, 1)

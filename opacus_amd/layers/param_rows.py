@@ -27,6 +27,13 @@ def parameter_rows(module: nn.Module, params: Sequence[nn.Parameter], n: int) ->
     return rows
 
 
+def rows_dim(module: nn.Module) -> int:
+    """The dimension of ``module``'s input that the samples lie along: 0, or 1 where the grad-sample hooks
+    of a model with ``batch_first=False`` are installed on a layer that follows the model's layout
+    (``follows_layout = True``). The rows themselves are samples first in either case."""
+    return module.__dict__.get("_dpk_rows_hooked", 0)
+
+
 def first_derivative_only(what: str) -> None:
     """Called inside a backward pass, where grad mode is on only under ``create_graph=True``: the
     kernels' gradients are not differentiable, and a graph over them would silently lack terms."""

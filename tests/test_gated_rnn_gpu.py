@@ -419,3 +419,59 @@ def test_large_rows_take_the_clipped_sum_from_the_rows_again():
         grads.append([p.grad.clone() for p in norm.parameters()])
     for p, q in zip(*grads):
         assert torch.equal(p, q) and p.abs().max() > 0
+
+
+class TimeFirst(nn.Module):
+    """``[T, B, 6]`` inputs; a layer of each kind that keeps the samples along the second dimension."""
+
+    def __init__(self):
+        super().__init__()
+        from opacus_amd.layers import HeadNormAct
+
+        self.inp, self.norm = nn.Linear(6, 24), HeadNormAct(4, 24, activation="gelu")
+        self.rnn = DPGatedRNN_(24, 24, 1, False, 3, False)
+        self.out = nn.Linear(24, 5)
+
+    def forward(self, x):
+        return self.out(self.rnn(self.norm(self.inp(x)))[0])  # [T, B, 5]
+
+    def reference(self, x):  # one sample [1, T, 6]
+        z = ref_norm(self.norm, F.linear(x, self.inp.weight, self.inp.bias))
+        return F.linear(ref_rnn(self.rnn, z)[0], self.out.weight, self.out.bias)
+
+
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("T", [7, 5])  # as many positions as samples, too
+def test_samples_along_the_second_dimension(T, reduction):
+    from opacus_amd import GradSampleModule, GradSampleModuleFastGradientClipping
+
+    torch.manual_seed(3)
+    net = TimeFirst()
+    with torch.no_grad():
+        for p in net.norm.parameters():
+            p.add_(0.3 * torch.randn(p.shape))
+    x, mask = torch.randn(T, 5, 6), torch.randn(T, 5, 5)
+    ref = copy.deepcopy(net).double()
+    rows = []
+    for k in range(5):
+        ref.zero_grad(set_to_none=True)
+        (ref.reference(x[:, k].double()[None])[0] * mask[:, k].double()).sum().backward()
+        rows.append({n: p.grad.clone() for n, p in ref.named_parameters()})
+    want = {n: torch.stack([r[n] for r in rows]) for n in rows[0]}
+    plain = copy.deepcopy(net).cuda()(x.cuda())
+    wrapped = GradSampleModule(copy.deepcopy(net).cuda(), batch_first=False, loss_reduction=reduction)
+    out = wrapped(x.cuda())
+    assert torch.equal(out, plain)
+    loss = (out * mask.cuda()).sum()
+    (loss / 5 if reduction == "mean" else loss).backward()
+    for name, p in wrapped._module.named_parameters():
+        assert_rel(p.grad_sample, want[name], REL, name)
+    ghost = GradSampleModuleFastGradientClipping(
+        copy.deepcopy(net).cuda(), batch_first=False, loss_reduction=reduction, max_grad_norm=1.0, use_ghost_clipping=True
+    )
+    loss = (ghost(x.cuda()) * mask.cuda()).sum()
+    (loss / 5 if reduction == "mean" else loss).backward()
+    norms = sum(w.flatten(1).square().sum(1) for w in want.values()).sqrt()
+    assert_rel(ghost.get_norm_sample()[None], norms[None], REL, "norms")
+    with pytest.raises(ValueError, match="batch_first=False"):
+        wrapped._module.norm(torch.zeros(5, 24, device="cuda"))
