@@ -97,6 +97,7 @@ __device__ __forceinline__ float inv_scale(float q2) { return __builtin_amdgcn_r
 // never depends on timing, so the bits repeat; the serial part of a row is one hop per run.
 // A word is 64 bits, stored and read whole at agent scope (the XCDs' L2s are not coherent), with
 // the pattern kEmpty in its low half until it is written; a NaN is published as the usual quiet one.
+// (One row of 128 tiles of 2048 channels: 68 us with runs of 16, 70 with 8, 32 or 64; two rows backward: 123, 125, 124, 132.)
 constexpr int kRun = 16;
 constexpr uint32_t kEmpty = 0xffffffffu;
 
