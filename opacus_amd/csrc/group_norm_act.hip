@@ -989,26 +989,36 @@ bool plan_rows(NormArgs* p, int dtype, bool backward, int* V, int* NI) {
   return true;
 }
 
-size_t part_bytes(int64_t n, int64_t S, int64_t C) {
+// A group of up to 256 channels fits a wave, whatever its alignment.
+bool wave_holds(int64_t C, int64_t G) { return C / G <= 4 * DPK_WAVE; }
+// The partial sums of the chunks, for whichever type and width the call has; nothing where the kernels
+// that need none run for all of them.
+size_t part_bytes(int64_t n, int64_t S, int64_t C, int64_t G, int per_position) {
+  const size_t chunk = static_cast<size_t>(n) * C * sizeof(float2);
   size_t most = 0;
-  for (int V = 1; V <= 8; V *= 2) {  // whichever width the pointers allow
-    if (C % V) break;
-    NormArgs p = {};
-    p.n = n, p.S = S, p.C = static_cast<int>(C);
-    plan(&p, V, true);
-    const size_t need = static_cast<size_t>(n) * p.J * C * sizeof(float2);
-    if (need > most) most = need;
+  if (per_position) {
+    // a sample is cut into no more chunks than 64-row ones, nor than it takes to fill the GPU
+    int64_t J = dpk_cdiv(S, 64);
+    if (J > dpk_cdiv(kWantBlocks, n)) J = dpk_cdiv(kWantBlocks, n);
+    if (J > 1) most = chunk * J;
   }
-  // statistics per position cut a sample into no more chunks than 64-row ones, nor than it takes to fill the GPU
-  int64_t J = dpk_cdiv(S, 64);
-  if (J > dpk_cdiv(kWantBlocks, n)) J = dpk_cdiv(kWantBlocks, n);
-  if (static_cast<size_t>(n) * J * C * sizeof(float2) > most) most = static_cast<size_t>(n) * J * C * sizeof(float2);
+  if (!per_position || !wave_holds(C, G)) {
+    for (int V = 1; V <= 8 && C % V == 0; V *= 2) {
+      NormArgs p = {};
+      p.n = n, p.S = S, p.C = static_cast<int>(C), p.G = static_cast<int>(G), p.Cg = p.C / p.G;
+      int R;
+      bool slabs = !per_position;
+      for (const int dtype : {DPK_BF16, DPK_F32})
+        if (V * dpk_elsize(dtype) <= 16) slabs = slabs && plan_slabs(&p, V, dtype, &R);
+      if (slabs) continue;
+      plan(&p, V, true);
+      if (chunk * p.J > most) most = chunk * p.J;
+    }
+  }
   return dpk_align_up(most, 256);
 }
-// (mean, rstd) of every position's groups where no wave may hold one (a group of up to 256 channels fits
-// whatever its alignment), or (S1, S2) of every sample's.
-size_t group_bytes(int64_t n, int64_t S, int64_t C, int64_t G, int per_position) {
-  if (per_position && C / G <= 4 * DPK_WAVE) return 0;
+// (mean, rstd) of every position's groups where no wave may hold one, or (S1, S2) of every sample's.
+size_t group_bytes(int64_t n, int64_t S, int64_t G, int per_position) {
   return dpk_align_up(static_cast<size_t>(n) * (per_position ? S : 1) * G * sizeof(float2), 256);
 }
 
@@ -1076,8 +1086,10 @@ void by_width(int dtype, int V, F&& body) {
 }  // namespace
 
 extern "C" size_t dpk_group_norm_act_workspace_bytes(int64_t n, int64_t S, int64_t C, int64_t groups, int per_position) {
-  if (n <= 0 || S <= 0 || C <= 0 || groups <= 0) return 0;
-  return part_bytes(n, S, C) + group_bytes(n, S, C, groups, per_position);
+  if (n <= 0 || S <= 0 || C <= 0 || groups <= 0 || C > (1 << 24) || C % groups) return 0;  // nothing to do, or refused
+  const size_t part = part_bytes(n, S, C, groups, per_position);
+  if (per_position ? wave_holds(C, groups) : part == 0) return part;
+  return part + group_bytes(n, S, groups, per_position);
 }
 
 extern "C" int dpk_group_norm_act(const void* x, int dtype, const void* weight, const void* bias, int param_dtype, void* y,
@@ -1169,7 +1181,7 @@ extern "C" int dpk_group_norm_act_backward(const void* x, const void* grad_out, 
   plan(&p, V, true);
   dim3 grid;
   if (int rc = grid_of(fn, p, &grid)) return rc;
-  float2* groups_ws = reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(n, S, C));
+  float2* groups_ws = reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(n, S, C, groups, per_position));
   if (per_position) {
     DPK_REQUIRE(dpk_grid_fits(dpk_cdiv(n * S * groups, kThreads / DPK_WAVE), kThreads), DPK_E_SHAPE, "%s: too large", fn);
     p.stats = groups_ws;

@@ -914,27 +914,34 @@ def _gates_layout(gates: torch.Tensor, D: int) -> Tuple[torch.Tensor, int, int]:
     return gates, (gates.stride(0) if n > 1 else T * 3 * D), (gates.stride(1) if T > 1 else 3 * D)
 
 
+def _float32_empty(like: torch.Tensor, *shape: int) -> torch.Tensor:
+    return like.new_empty(*shape) if like.dtype is torch.float32 else like.new_empty(shape, dtype=torch.float32)
+
+
 def _scan_args(gates, decay, lengths, dims: int):
+    """The device, the sizes ``(n, T, D)`` (T 1 for two dimensions), decay and lengths dense, and the
+    dtypes of gates and decay."""
     dev = _need_gpu(gates, decay, lengths)
-    if gates.dim() != dims:
-        raise ValueError(f"gates must have {dims} dimensions, got {tuple(gates.shape)}")
-    if decay.dim() != 1 or gates.shape[-1] != 3 * decay.shape[0]:
-        raise ValueError(f"gates {tuple(gates.shape)} must end in 3 * D features for decay {tuple(decay.shape)}")
-    _code(gates), _code(decay)
+    shape = gates.shape
+    if len(shape) != dims:
+        raise ValueError(f"gates must have {dims} dimensions, got {tuple(shape)}")
+    if decay.dim() != 1 or shape[-1] != 3 * decay.shape[0]:
+        raise ValueError(f"gates {tuple(shape)} must end in 3 * D features for decay {tuple(decay.shape)}")
     if lengths is not None:
-        if lengths.dtype != torch.int64 or tuple(lengths.shape) != (gates.shape[0],):
-            raise ValueError(f"lengths must be int64 of shape ({gates.shape[0]},), got {lengths.dtype} {tuple(lengths.shape)}")
+        if lengths.dtype != torch.int64 or lengths.shape != shape[:1]:
+            raise ValueError(f"lengths must be int64 of shape ({shape[0]},), got {lengths.dtype} {tuple(lengths.shape)}")
         lengths = _dense(lengths)
-    return dev, _dense(decay), lengths
+    sizes = (shape[0], shape[1] if dims == 3 else 1, shape[-1] // 3)
+    return dev, sizes, _dense(decay), lengths, _code(gates), _code(decay)
 
 
-def _scan_state(name: str, t: Optional[torch.Tensor], shape, dev) -> Optional[torch.Tensor]:
+def _scan_state(name: str, t: Optional[torch.Tensor], shape: Tuple[int, ...], dev) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if _need_gpu(t) != dev:
+    if t.device != dev:
         raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
-    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be float32 of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype is not torch.float32 or t.shape != shape:
+        raise ValueError(f"{name} must be float32 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     return _dense(t)
 
 
@@ -956,12 +963,11 @@ def gated_scan(
     positions from ``lengths[b]`` on as padding, which is never read: the state passes over it and
     the output is zero there. ``reverse`` scans from the last position to the first. ``gates``
     may be a slice of a larger tensor (any strides but along the features)."""
-    dev, decay, lengths = _scan_args(gates, decay, lengths, 3)
-    n, T, D = gates.shape[0], gates.shape[1], decay.shape[0]
+    dev, (n, T, D), decay, lengths, code, decay_code = _scan_args(gates, decay, lengths, 3)
     state = _scan_state("state", state, (n, D), dev)
-    out = torch.empty((n, T, D), dtype=gates.dtype, device=dev)
-    last = torch.empty((n, D), dtype=torch.float32, device=dev)
-    kept = torch.empty((n, -(-T // _lib.DPK_SCAN_CHUNK), D), dtype=torch.float32, device=dev) if keep_states else None
+    out = gates.new_empty(n, T, D)
+    last = _float32_empty(decay, n, D)
+    kept = _float32_empty(decay, n, -(-T // _lib.DPK_SCAN_CHUNK), D) if keep_states else None
     if n == 0 or D == 0:
         return out, last, kept
     gates, sn, st = _gates_layout(gates, D)
@@ -969,7 +975,7 @@ def gated_scan(
     ws, wsb = _ws(L.dpk_gated_scan_workspace_bytes(n, T, D), dev)
     _launch(
         "dpk_gated_scan", dev,
-        _at(gates), _code(gates), _at(decay), _code(decay), _at(state), _at(lengths), _at(out), _at(last),
+        _at(gates), code, _at(decay), decay_code, _at(state), _at(lengths), _at(out), _at(last),
         _at(kept), n, T, D, sn, st, int(bool(reverse)), _at(ws), wsb,
     )
     return out, last, kept
@@ -989,18 +995,17 @@ def gated_scan_backward(
     ``decay``: the pass that forms the gate gradients has it on the way. ``kept`` is what
     ``gated_scan(..., keep_states=True)`` returned for the same gates, decay, lengths and direction;
     ``grad_last`` (float32) is the gradient of the last state."""
-    dev, decay, lengths = _scan_args(gates, decay, lengths, 3)
-    n, T, D = gates.shape[0], gates.shape[1], decay.shape[0]
+    dev, (n, T, D), decay, lengths, code, decay_code = _scan_args(gates, decay, lengths, 3)
     _need_gpu(gates, kept, grad_out)
-    if tuple(grad_out.shape) != (n, T, D):
+    if grad_out.shape != (n, T, D):
         raise ValueError(f"grad_out must be {(n, T, D)}, got {tuple(grad_out.shape)}")
     if grad_out.dtype != gates.dtype:
         grad_out = grad_out.to(gates.dtype)
     kept = _scan_state("kept", kept, (n, -(-T // _lib.DPK_SCAN_CHUNK), D), dev)
     grad_last = _scan_state("grad_last", grad_last, (n, D), dev)
-    grad_gates = torch.empty((n, T, 3 * D), dtype=gates.dtype, device=dev)
-    grad_decay = torch.empty((n, D), dtype=torch.float32, device=dev)
-    grad_state = torch.empty((n, D), dtype=torch.float32, device=dev)
+    grad_gates = gates.new_empty(n, T, 3 * D)
+    grad_decay = kept.new_empty(n, D)
+    grad_state = kept.new_empty(n, D)
     if n == 0 or D == 0:
         return grad_gates, grad_decay, grad_state
     gates, sn, st = _gates_layout(gates, D)
@@ -1009,7 +1014,7 @@ def gated_scan_backward(
     ws, wsb = _ws(L.dpk_gated_scan_workspace_bytes(n, T, D), dev)
     _launch(
         "dpk_gated_scan_backward", dev,
-        _at(gates), _code(gates), _at(decay), _code(decay), _at(kept), _at(lengths), _at(grad_out),
+        _at(gates), code, _at(decay), decay_code, _at(kept), _at(lengths), _at(grad_out),
         _at(grad_last), _at(grad_gates), _at(grad_decay), _at(grad_state), n, T, D, sn, st,
         int(bool(reverse)), _at(ws), wsb,
     )
@@ -1019,21 +1024,20 @@ def gated_scan_backward(
 def gated_scan_step(gates: torch.Tensor, decay: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     """One position of :func:`gated_scan`: ``gates`` ``[n, 3 D]``; ``state`` (dense float32
     ``[n, D]``) is advanced in place and returned rounded to the gates' dtype."""
-    dev, decay, _ = _scan_args(gates, decay, None, 2)
-    n, D = gates.shape[0], decay.shape[0]
+    dev, (n, _, D), decay, _, code, decay_code = _scan_args(gates, decay, None, 2)
     if not state.is_contiguous():
         raise ValueError("state is advanced in place and must be dense")
     if state.requires_grad and torch.is_grad_enabled():
         raise ValueError("gated_scan_step advances its state in place and is not differentiable: use gated_scan")
     _scan_state("state", state, (n, D), dev)
-    out = torch.empty((n, D), dtype=gates.dtype, device=dev)
+    out = gates.new_empty(n, D)
     if n == 0 or D == 0:
         return out
     if gates.stride(1) != 1 or gates.stride(0) < 0:
         gates = gates.contiguous()
     _launch(
         "dpk_gated_scan_step", dev,
-        _at(gates), _code(gates), _at(decay), _code(decay), _at(state), _at(out), n, D,
+        _at(gates), code, _at(decay), decay_code, _at(state), _at(out), n, D,
         gates.stride(0) if n > 1 else 3 * D,
     )
     if not state.is_inference():  # (tensors made in inference mode have no version to count)
@@ -1053,15 +1057,16 @@ def _norm_act_args(x, num_groups, weight, bias, eps, activation):
         raise ValueError(f"activation must be one of {sorted(_lib.DPK_ACT)}, got {activation!r}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    _code(x)
-    params = [p for p in (weight, bias) if p is not None]
-    for p in params:
-        if tuple(p.shape) != (C,):
-            raise ValueError(f"weight and bias must have shape ({C},), got {tuple(p.shape)}")
-    if len(params) == 2 and weight.dtype != bias.dtype:
+    pcode = DPK_F32
+    for p in (weight, bias):
+        if p is not None:
+            if p.shape != (C,):
+                raise ValueError(f"weight and bias must have shape ({C},), got {tuple(p.shape)}")
+            pcode = _code(p)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias differ in dtype: {weight.dtype} and {bias.dtype}")
-    weight, bias = (None if p is None else _dense(p) for p in (weight, bias))
-    return dev, weight, bias, (_code(params[0]) if params else DPK_F32)
+    weight, bias = None if weight is None else _dense(weight), None if bias is None else _dense(bias)
+    return dev, weight, bias, _code(x), pcode
 
 
 def group_norm_act(
@@ -1078,19 +1083,19 @@ def group_norm_act(
     channels run over all positions of the sample (``nn.GroupNorm``), or with ``per_position`` over
     each position alone (the heads of a token). Returns ``(y, stats)``; ``stats`` (None with
     ``per_position``) goes to :func:`group_norm_act_backward`."""
-    dev, weight, bias, pcode = _norm_act_args(x, num_groups, weight, bias, eps, activation)
+    dev, weight, bias, code, pcode = _norm_act_args(x, num_groups, weight, bias, eps, activation)
     x = _dense(x)
     n, C = x.shape[0], x.shape[-1]
     S = math.prod(x.shape[1:-1])
     y = torch.empty_like(x)
-    stats = None if per_position else torch.empty((n, num_groups, 2), dtype=torch.float32, device=dev)
+    stats = None if per_position else _float32_empty(x if weight is None else weight, n, num_groups, 2)
     if n == 0 or S == 0:
         return y, stats
     L = lib()
     ws, wsb = _ws(L.dpk_group_norm_act_workspace_bytes(n, S, C, num_groups, int(bool(per_position))), dev)
     _launch(
         "dpk_group_norm_act", dev,
-        _at(x), _code(x), _at(weight), _at(bias), pcode, _at(y), _at(stats), n, S, C, num_groups, float(eps),
+        _at(x), code, _at(weight), _at(bias), pcode, _at(y), _at(stats), n, S, C, num_groups, float(eps),
         _lib.DPK_ACT[activation], int(bool(per_position)), _at(ws), wsb,
     )
     return y, stats
@@ -1110,7 +1115,7 @@ def group_norm_act_backward(
     """Gradients of :func:`group_norm_act`: ``(grad_x, grad_weight [n, C], grad_bias [n, C])``. The
     last two (float32) are the per-sample gradients; the pass over ``x`` and ``grad_out`` that the
     input gradient needs has them on the way."""
-    dev, weight, bias, pcode = _norm_act_args(x, num_groups, weight, bias, eps, activation)
+    dev, weight, bias, code, pcode = _norm_act_args(x, num_groups, weight, bias, eps, activation)
     _need_gpu(x, grad_out, stats)
     if grad_out.shape != x.shape:
         raise ValueError(f"grad_out must be {tuple(x.shape)}, got {tuple(grad_out.shape)}")
@@ -1120,7 +1125,7 @@ def group_norm_act_backward(
     n, C = x.shape[0], x.shape[-1]
     S = math.prod(x.shape[1:-1])
     if not per_position:
-        if stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (n, num_groups, 2):
+        if stats is None or stats.dtype != torch.float32 or stats.shape != (n, num_groups, 2):
             raise ValueError(f"stats must be what group_norm_act returned, float32 {(n, num_groups, 2)}")
         stats = _dense(stats)
     else:
@@ -1128,13 +1133,13 @@ def group_norm_act_backward(
     grad_x = torch.empty_like(x)
     if n == 0 or S == 0:
         return grad_x, *(torch.zeros((n, C), dtype=torch.float32, device=dev) for _ in range(2))
-    grad_w = torch.empty((n, C), dtype=torch.float32, device=dev)
-    grad_b = torch.empty((n, C), dtype=torch.float32, device=dev)
+    grad_w = _float32_empty(x if weight is None else weight, n, C)
+    grad_b = torch.empty_like(grad_w)
     L = lib()
     ws, wsb = _ws(L.dpk_group_norm_act_workspace_bytes(n, S, C, num_groups, int(bool(per_position))), dev)
     _launch(
         "dpk_group_norm_act_backward", dev,
-        _at(x), _at(grad_out), _code(x), _at(weight), _at(bias), pcode, _at(stats), _at(grad_x), _at(grad_w),
+        _at(x), _at(grad_out), code, _at(weight), _at(bias), pcode, _at(stats), _at(grad_x), _at(grad_w),
         _at(grad_b), n, S, C, num_groups, float(eps), _lib.DPK_ACT[activation], int(bool(per_position)),
         _at(ws), wsb,
     )

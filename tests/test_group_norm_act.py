@@ -57,11 +57,17 @@ def test_c_entry_points_refuse_before_any_launch():
         assert call(act=4) == ARG and call(act=-1) == ARG and call(pp=2) == ARG and call(eps=-1.0) == ARG
         assert call(eps=float("nan")) == ARG and call(x=None) == ARG and call(y=None) == ARG and call(stats=None) == ARG
         assert call(x=one + 2) == ALIGN and call(w=one + 1) == ALIGN and call(stats=one + 4) == ALIGN
-        assert call(ws=None) == WS and call(wsb=0) == WS and call(ws=one + 8) == ALIGN
+        for k in (dict(S=10**6), dict(S=10**6, pp=1)):
+            assert call(ws=None, **k) == WS and call(wsb=0, **k) == WS
+        assert call(ws=one + 8) == ALIGN
         assert call(n=0) == 0 and call(S=0) == 0
         assert b"group_norm_act" in L.dpk_last_error()
     assert bwd(dy=None) == ARG
-    assert L.dpk_group_norm_act_workspace_bytes(0, 4, 8, 2, 0) == 0
+    need = L.dpk_group_norm_act_workspace_bytes
+    assert need(0, 4, 8, 2, 0) == 0 and need(1, 4, 8, 2**32, 0) == 0 and need(1, 4, 2**40, 2, 0) == 0
+    # none where a block holds a sample's groups, or a wave a position's and a sample is one chunk
+    assert need(33, 49, 210, 14, 0) == 0 and need(64, 64, 2048, 16, 1) == 0
+    assert need(3, 40000, 128, 32, 0) > 0 and need(16, 1024, 2048, 16, 1) > 0 and need(2, 4, 600, 1, 1) > 0
 
 
 @pytest.mark.parametrize(
