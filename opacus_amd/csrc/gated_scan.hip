@@ -7,8 +7,8 @@
 // The recurrence is a composition of affine maps h -> A h + B, so T is cut at will. A block takes one
 // tile of positions for 32 * V channels of a sample: every thread runs K positions of its channels in
 // registers, the block's time groups exchange their (A, B) through lanes and LDS, and the tiles of a
-// row pass the state on in one launch (see "the chain" below), so every input is read once and every
-// output written once. What is folded, and in which order, depends on sizes alone: the same bits on
+// row pass the state on in one launch (see "the chain" below), or one block walks through all of them where
+// that is faster (bwd_walks), so every input is read once and every output written once. What is folded, and in which order, depends on sizes alone: the same bits on
 // every run.
 //
 // Backward: g_t = dy_t + a_{t+1} g_{t+1} runs the same maps the other way (same A, other B), and
@@ -21,13 +21,14 @@
 // enters a gradient.
 //
 // Bounds, at 16 x 1024 x 2048: forward bf16 54 us for 272 MB (5.0 TB/s; a large copy reaches 4.9 to 5.3), fp32 110 us
-// for 541 MB (4.9 TB/s): memory. Backward fp32 200 us for 948 MB (4.7 TB/s): memory. Backward bf16 118 us for 478 MB
-// (4.1 TB/s), about 10 us of them the chain's clearing and the sum of the decay gradients: half the
-// cycles issue arithmetic (62 vector instructions an element, 6 of them transcendental), and three waves
-// a SIMD are what their registers leave to cover loads with. Tried for it and slower: 4 positions a thread
-// in blocks of 512 (four waves a SIMD, 130 us), two waves with nothing spilled (134 us), four with spills
-// (211 us against 126 then), two rows a block with the second one's inputs sent ahead into LDS (140 us
-// against 126 then). One 16384-token row of 2048 channels: 68 us for 268 MB; a summary launch in front
+// for 541 MB (4.9 TB/s): memory. Backward fp32 187 us for 948 MB (5.1 TB/s): memory. Backward bf16 109 us for 478 MB
+// (4.4 TB/s): half the cycles issue arithmetic (62 vector instructions an element, 6 of them transcendental),
+// and the two waves a SIMD that their registers leave cover the loads for the rest. There a block walks; in the
+// chain it is 119 us, about 10 of them its clearing and the sum of the decay gradients. Tried for the walk and
+// slower: the next tile's inputs sent ahead into registers (116 us, fp32 242), three waves (129 us). For the chain:
+// 4 positions a thread in blocks of 512 (four waves a SIMD, 130 us), two waves with nothing spilled (134 us),
+// four with spills (211 us against 126 then), two rows a block with the second one's inputs sent ahead into
+// LDS (140 us against 126 then). One 16384-token row of 2048 channels: 68 us for 268 MB; a summary launch in front
 // instead of the chain took 127 us.
 #include <initializer_list>
 
@@ -41,7 +42,8 @@ constexpr int kCL = 32;                  // lanes across channels: a wave holds 
 constexpr int kChunk = DPK_SCAN_CHUNK;   // positions between kept states
 constexpr int kBwdK = 8;                 // positions per thread
 constexpr int kBwdTile = kBwdThreads / kCL * kBwdK;  // 64
-constexpr int kFwdTile = 128;            // forward: 16 positions per thread, or 8 where T is 64 at most
+constexpr int kFwdTile = 128;            // forward: 16 positions per thread, or 8 where T is 64 at most or a block walks
+constexpr int kWalkTile = 64;
 static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0, "tiles start at kept states");
 // Byte offsets inside a tile are 32 bits wide.
 constexpr int64_t kMaxStride = (1LL << 31) / (kFwdTile * 4) - 1;
@@ -202,6 +204,23 @@ __device__ __forceinline__ void state_before(const Chain& ch, int64_t row, int t
   }
 }
 
+// The same for a block that walks a row: the state lies in LDS from one tile to the next. Every thread has
+// passed a barrier since the last tile's owner wrote it, and passes the one here before the next tile's
+// maps overwrite what it folded.
+template <int V>
+__device__ __forceinline__ void pass_state(int t, int cw, bool owner, const float (&TA)[V], const float (&TB)[V], float (&in)[V],
+                                           float* lds_s) {
+  if (t > 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) in[j] = lds_s[cw + j];
+  }
+  __syncthreads();
+  if (owner) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds_s[cw + j] = fmaf(TA[j], in[j], TB[j]);
+  }
+}
+
 struct ScanArgs {
   const void* gates;
   const void* decay;
@@ -224,7 +243,7 @@ struct ScanBwdArgs {
   const float* dlast;      // [n,D] or null
   void* dgates;            // [n,T,3D]
   float* dstate;           // [n,D] or null
-  float* dlam;             // [tiles,n,D] (the result itself if there is one tile) or null
+  float* dlam;             // [tiles,n,D] (the result itself if a block takes the whole row) or null
   int64_t n, T, D, sn, st;
   int decay_bf16, reverse;
   Chain ch;
@@ -329,8 +348,9 @@ __device__ __forceinline__ void fold_waves(const float (*la)[kCL * V], const flo
   }
 }
 
-// FULL: every position and channel of the tile is live.
-template <typename T, int V, int K, bool FULL>
+// FULL: every position and channel of the tile is live. WALK: the block takes the tiles of its row one after the
+// other, and the state between them lies in lds_s.
+template <typename T, int V, int K, bool FULL, bool WALK>
 __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
                                          const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
@@ -360,7 +380,7 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
   const int64_t row = b * p.D + c;
   float h[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) h[j] = on && p.state && t < kRun ? p.state[row + j] : 0.f;
+  for (int j = 0; j < V; ++j) h[j] = on && p.state && t < (WALK ? 1 : kRun) ? p.state[row + j] : 0.f;
   float a[K][V], u[K][V], A[V], B[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) A[j] = 1.f, B[j] = 0.f;
@@ -393,8 +413,12 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
   const bool owner = wave == kWaves - 1 && !late;
 #pragma unroll
   for (int j = 0; j < V; ++j) TB[j] = fmaf(TA[j], PB[j], TB[j]), TA[j] *= PA[j];  // the tile's map, in the last wave
-  publish_map<V>(p.ch, r, t, cl, owner, TA, TB);
-  state_before<V, kThreads / kCL>(p.ch, r, t, cl, tg, owner, TA, TB, h, lds_m, lds_s);
+  if (WALK) {
+    pass_state<V>(t, cw, owner, TA, TB, h, lds_s);
+  } else {
+    publish_map<V>(p.ch, r, t, cl, owner, TA, TB);
+    state_before<V, kThreads / kCL>(p.ch, r, t, cl, tg, owner, TA, TB, h, lds_m, lds_s);
+  }
   if (on && owner && t + 1 == p.ch.tiles) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.last[row + j] = fmaf(TA[j], h[j], TB[j]);
@@ -425,31 +449,37 @@ __device__ __forceinline__ void fwd_tile(const ScanArgs& p, int t, int64_t r, in
   }
 }
 
-// One block: one tile of 8 * K positions of 32 * V channels of one sample.
-template <typename T, int V, int K>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void scan_fwd_kernel(ScanArgs p) {
+// One block: one tile of 8 * K positions of 32 * V channels of one sample, or (WALK) all of them in turn.
+template <typename T, int V, int K, bool WALK>
+__global__ __launch_bounds__(kThreads, WALK ? 2 : sizeof(T) == 2 ? 4 : 3) void scan_fwd_kernel(ScanArgs p) {
   constexpr int W = kCL * V, kWaves = kThreads / DPK_WAVE, TILE = kThreads / kCL * K;
   static_assert(TILE % kChunk == 0 && kChunk % K == 0, "a time group starts where a state is kept");
   __shared__ float lds_a[kWaves][W];
   __shared__ float lds_b[kWaves][W];
-  __shared__ float lds_m[2 * kRun * W];
+  __shared__ float lds_m[WALK ? 1 : 2 * kRun * W];
   __shared__ float lds_s[W];
   __shared__ int lds_t;
   const int64_t cbs = (p.D + W - 1) / W, r = row_of<T>(p.ch.rows), b = r / cbs, cb = r - b * cbs;
-  draw_tile(p.ch, r, &lds_t);
+  if (!WALK) draw_tile(p.ch, r, &lds_t);
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
-  const int t = drawn_tile(&lds_t);
+  int t = WALK ? 0 : drawn_tile(&lds_t);
   if (t >= p.ch.tiles) return;  // never, unless another call used the workspace meanwhile
-  const Tile tl = tile_of<TILE>(p.T, live_length(p.lengths, b, p.T), static_cast<int64_t>(t) * TILE, p.reverse);
-  if (tl.hi - tl.lo == TILE && (cb + 1) * W <= p.D) fwd_tile<T, V, K, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
-  else fwd_tile<T, V, K, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
+  const int64_t len = live_length(p.lengths, b, p.T);
+  do {
+    const Tile tl = tile_of<TILE>(p.T, len, static_cast<int64_t>(t) * TILE, p.reverse);
+    if (tl.hi - tl.lo == TILE && (cb + 1) * W <= p.D)
+      fwd_tile<T, V, K, true, WALK>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
+    else
+      fwd_tile<T, V, K, false, WALK>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_m, lds_s);
+  } while (WALK && ++t < p.ch.tiles);
 }
 
-template <typename T, int V, bool FULL>
+// acc: this thread's share of the decay's gradient, over its tiles.
+template <typename T, int V, bool FULL, bool WALK>
 __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r, int64_t b, int64_t cb, const Tile& tl,
-                                         const float (&sp)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V], float (*lds_g)[kCL * V],
-                                         float* lds_m, float* lds_s) {
+                                         const float (&sp)[V], float (&acc)[V], float (*lds_a)[kCL * V], float (*lds_b)[kCL * V],
+                                         float (*lds_g)[kCL * V], float* lds_m, float* lds_s) {
   typedef vec_io<T, V> io;
   constexpr int W = kCL * V, K = kBwdK, E = sizeof(T), kWaves = kBwdThreads / DPK_WAVE;
   const int cl = threadIdx.x % kCL, tg = threadIdx.x / kCL;
@@ -478,14 +508,14 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
       rd[k] = load_at<T, V>(dy + at1, q1);
     }
   }
-  const int64_t nD = p.n * p.D, row = b * p.D + c;
+  const int64_t row = b * p.D + c;
   float h[V], g[V];
   typename vec_io<float, V>::raw kh = typename vec_io<float, V>::raw();
   if (on && p.T > 0) kh = vec_io<float, V>::load(p.kept + (b * p.ch.tiles + tile) * p.D + c);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     h[j] = vec_io<float, V>::get(kh, j);
-    g[j] = on && p.dlast && t < kRun ? p.dlast[row + j] : 0.f;
+    g[j] = on && p.dlast && t < (WALK ? 1 : kRun) ? p.dlast[row + j] : 0.f;
   }
   // what the second half needs of each element; the rest is a product or two away
   float a[K][V], ms[K][V], is[K][V], sg[K][V], rho[K][V];  // ms = m s, is = s / m
@@ -537,7 +567,7 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
   const bool owner = wave == 0 && !late;
 #pragma unroll
   for (int j = 0; j < V; ++j) TG[j] = fmaf(TA[j], PG[j], TG[j]), TA[j] *= PA[j];
-  publish_map<V>(p.ch, r, t, cl, owner, TA, TG);
+  if (!WALK) publish_map<V>(p.ch, r, t, cl, owner, TA, TG);
   // the states inside the tile, while the words of the chain are on their way
   for (int w = 0; w < wave; ++w) {
 #pragma unroll
@@ -552,9 +582,7 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
 #pragma unroll
     for (int j = 0; j < V; ++j) asm volatile("" : "+v"(ms[k][j]), "+v"(sg[k][j]), "+v"(rho[k][j]), "+v"(is[k][j]));
   }
-  float hp[K][V], acc[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  float hp[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -563,7 +591,8 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
       h[j] = fmaf(a[k][j], h[j], ms[k][j] * io::get(rx[k], j));
     }
   }
-  state_before<V, kBwdThreads / kCL>(p.ch, r, t, cl, tg, owner, TA, TG, g, lds_m, lds_s);
+  if (WALK) pass_state<V>(t, cw, owner, TA, TG, g, lds_s);
+  else state_before<V, kBwdThreads / kCL>(p.ch, r, t, cl, tg, owner, TA, TG, g, lds_m, lds_s);
   if (on && owner && p.dstate && tile == 0) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.dstate[row + j] = fmaf(TA[j], g[j], TG[j]);
@@ -602,8 +631,14 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
       store_at<T, V>(di + at, q, oi);
     }
   }
-  if (!p.dlam) return;
-  // sum_t of the tile over the time groups, in order
+}
+
+// The decay's gradient of the block's tiles, `to` [n,D]: acc summed over the time groups, in order.
+template <int V>
+__device__ __forceinline__ void store_decay_sums(const ScanBwdArgs& p, float* to, int64_t b, int c, const float (&sp)[V],
+                                                 const float (&acc)[V], float (*lds_g)[kCL * V]) {
+  const int cw = threadIdx.x % kCL * V, wave = threadIdx.x / DPK_WAVE;
+  const bool late = threadIdx.x / kCL & 1;
   float other[V];
   other_group<V>(acc, other);
   __syncthreads();
@@ -612,41 +647,50 @@ __device__ __forceinline__ void bwd_tile(const ScanBwdArgs& p, int t, int64_t r,
     for (int j = 0; j < V; ++j) lds_g[wave][cw + j] = acc[j] + other[j];
   }
   __syncthreads();
-  if (on && owner) {
+  if (c < p.D && wave == 0 && !late) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) sum += lds_g[w][cw + j];
+      for (int w = 0; w < kBwdThreads / DPK_WAVE; ++w) sum += lds_g[w][cw + j];
       // v lacks the factor -softplus(lam) of w, and dlam = sigma(lam) / softplus(lam) sum_t w;
       // sigma(lam) = 1 - exp(-softplus(lam))
-      p.dlam[tile * nD + row + j] = expm1f(-sp[j]) * sum;
+      to[b * p.D + c + j] = expm1f(-sp[j]) * sum;
     }
   }
 }
 
-// One block: one tile of 64 positions, from the row's last to its first.
-template <typename T, int V>
-__global__ __launch_bounds__(kBwdThreads, 3) void scan_bwd_kernel(ScanBwdArgs p) {
+// One block: one tile of 64 positions, or (WALK) all of them in turn, from the row's last to its first.
+template <typename T, int V, bool WALK>
+__global__ __launch_bounds__(kBwdThreads, WALK ? 2 : 3) void scan_bwd_kernel(ScanBwdArgs p) {
   constexpr int W = kCL * V, kWaves = kBwdThreads / DPK_WAVE;
   __shared__ float lds_a[kWaves][W];
   __shared__ float lds_b[kWaves][W];
   __shared__ float lds_g[kWaves][W];
-  __shared__ float lds_m[2 * kRun * W];
+  __shared__ float lds_m[WALK ? 1 : 2 * kRun * W];
   __shared__ float lds_s[W];
   __shared__ int lds_t;
   const int64_t cbs = (p.D + W - 1) / W, r = row_of<T>(p.ch.rows), b = r / cbs, cb = r - b * cbs;
-  draw_tile(p.ch, r, &lds_t);
+  if (!WALK) draw_tile(p.ch, r, &lds_t);
   float sp[V];
   softplus_of<V>(p.decay, p.decay_bf16, p.D, cb * W + (threadIdx.x % kCL) * V, sp);
-  const int t = drawn_tile(&lds_t);  // 0 is the last tile of the scan
+  int t = WALK ? 0 : drawn_tile(&lds_t);  // 0 is the last tile of the scan
   if (t >= p.ch.tiles) return;  // never, unless another call used the workspace meanwhile
-  const Tile tl = tile_of<kBwdTile>(p.T, live_length(p.lengths, b, p.T),
-                                    static_cast<int64_t>(p.ch.tiles - 1 - t) * kBwdTile, p.reverse);
-  if (tl.hi - tl.lo == kBwdTile && (cb + 1) * W <= p.D)
-    bwd_tile<T, V, true>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_g, lds_m, lds_s);
-  else
-    bwd_tile<T, V, false>(p, t, r, b, cb, tl, sp, lds_a, lds_b, lds_g, lds_m, lds_s);
+  const int64_t len = live_length(p.lengths, b, p.T);
+  float acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  do {
+    const Tile tl = tile_of<kBwdTile>(p.T, len, static_cast<int64_t>(p.ch.tiles - 1 - t) * kBwdTile, p.reverse);
+    if (tl.hi - tl.lo == kBwdTile && (cb + 1) * W <= p.D)
+      bwd_tile<T, V, true, WALK>(p, t, r, b, cb, tl, sp, acc, lds_a, lds_b, lds_g, lds_m, lds_s);
+    else
+      bwd_tile<T, V, false, WALK>(p, t, r, b, cb, tl, sp, acc, lds_a, lds_b, lds_g, lds_m, lds_s);
+  } while (WALK && ++t < p.ch.tiles);
+  if (p.dlam) {
+    float* to = p.dlam + (WALK ? 0 : (p.ch.tiles - 1 - t) * p.n * p.D);
+    store_decay_sums<V>(p, to, b, static_cast<int>(cb * W) + threadIdx.x % kCL * V, sp, acc, lds_g);
+  }
 }
 
 // out[i] = sum over the tiles of part[tile][i], in order: 64 sums a block, its 16 waves on 16 neighbouring
@@ -706,12 +750,12 @@ size_t chain_bytes(int64_t n, int64_t D, int V, int tiles) {
   const size_t rows = static_cast<size_t>(n * dpk_cdiv(D, kCL * V));
   return dpk_align_up(rows * 4, 256) + rows * kCL * V * 8 * (tiles + dpk_cdiv(tiles, kRun));
 }
-// Sets up and clears the chain of a launch; returns the first byte behind it.
-char* chain_of(Chain* ch, int64_t n, int64_t D, int V, int tiles, void* ws, hipStream_t s) {
+// Sets up and, but where blocks walk, clears the chain of a launch; returns the first byte behind it.
+char* chain_of(Chain* ch, int64_t n, int64_t D, int V, int tiles, bool walk, void* ws, hipStream_t s) {
   ch->rows = n * dpk_cdiv(D, kCL * V);
   ch->tiles = tiles;
   ch->runs = static_cast<int>(dpk_cdiv(tiles, kRun));
-  if (tiles == 1) return static_cast<char*>(ws);
+  if (tiles == 1 || walk) return static_cast<char*>(ws);
   const int64_t W = kCL * V, words = ch->rows * W * (tiles + ch->runs);
   char* at = static_cast<char*>(ws);
   ch->tickets = reinterpret_cast<uint32_t*>(at);
@@ -722,6 +766,19 @@ char* chain_of(Chain* ch, int64_t n, int64_t D, int V, int tiles, void* ws, hipS
   hipLaunchKernelGGL(chain_clear_kernel, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(kThreads), 0, s,
                      ch->tickets, ch->rows, reinterpret_cast<uint4*>(ch->maps), words / 2);
   return at + words * 8;
+}
+
+// Where one block takes all tiles of its row in turn, and no chain is set up. Few tiles: two launches and the
+// workspace saved are more than the tiles one after the other cost (us in a loop of calls, chain and walk: forward
+// 8 x 256 x 512 fp32 15.8 and 13.0, 64 x 192 x 1024 bf16 30.7 and 21.4, 7 x 333 x 130 fp32 15.8 and 20.6;
+// backward 8 x 192 x 512 fp32 19.3 and 14.5, 8 x 256 x 512 19.4 and 18.2, 7 x 333 x 130 19.1 and 25.5).
+// Backward also where rows fill the GPU's 512 places for such blocks to 85 % or more, whatever T: they lose nothing by
+// waiting for one another (16 x 1024 x 2048 bf16 119 and 109, fp32 201 and 187, 64 x 4096 x 500 bf16 483 and 416;
+// but half the rows, 8 x 1024 x 2048 bf16, 54 and 57, and three quarters of the places, 24 x 512 x 2048, 87 and 92).
+bool fwd_walks(int64_t T) { return T > kFwdTile && T <= 4 * kWalkTile; }
+bool bwd_walks(int64_t n, int64_t T, int64_t D) {
+  const int64_t rows = n * dpk_cdiv(D, 2 * kCL), places = dpk_cdiv(rows, 512) * 512;
+  return T > kBwdTile && (T <= 3 * kBwdTile || 20 * rows >= 17 * places);
 }
 
 int vec_of(int most, int64_t D, int dtype, int64_t sn, int64_t st, int64_t n, int64_t T, std::initializer_list<const void*> elems,
@@ -758,7 +815,7 @@ int check_common(const char* fn, const void* gates, int dtype, const void* decay
 }  // namespace
 
 extern "C" size_t dpk_gated_scan_workspace_bytes(int64_t n, int64_t T, int64_t D) {
-  if (n <= 0 || T <= kBwdTile || D <= 0) return 0;
+  if (n <= 0 || T <= kBwdTile || D <= 0 || ((T <= kFwdTile || fwd_walks(T)) && bwd_walks(n, T, D))) return 0;
   const int tiles = tiles_of(T, kBwdTile);  // the backward pass cuts finer
   size_t most = 0;
   for (int V = 1; V <= 2; V *= 2) {  // whichever width the pointers allow
@@ -781,22 +838,24 @@ extern "C" int dpk_gated_scan(const void* gates, int dtype, const void* decay, i
                   dpk_aligned(lengths, 8),
               DPK_E_ALIGN, "%s: a tensor is not aligned to its element size", fn);
   const int V = vec_of(2, D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, out}, {last, state, kept});
-  const int tiles = tiles_of(T, kFwdTile);
+  const bool walk = fwd_walks(T);
+  const int tiles = tiles_of(T, walk ? kWalkTile : kFwdTile);
   DPK_REQUIRE(dpk_grid_fits(n * dpk_cdiv(D, kCL * V) * tiles, kThreads), DPK_E_SHAPE, "%s: n * T * D too large", fn);
-  const size_t need = chain_bytes(n, D, V, tiles);
+  const size_t need = walk ? 0 : chain_bytes(n, D, V, tiles);
   DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
   DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
   hipStream_t s = static_cast<hipStream_t>(stream);
   ScanArgs p = {gates, decay, state, lengths, out, last, kept, n, T, D, gates_stride_n, gates_stride_t,
                 decay_dtype == DPK_BF16, reverse, {}};
-  chain_of(&p.ch, n, D, V, tiles, ws, s);
-  const dim3 grid(static_cast<unsigned>(p.ch.rows * tiles));
+  chain_of(&p.ch, n, D, V, tiles, walk, ws, s);
+  const dim3 grid(static_cast<unsigned>(p.ch.rows * (walk ? 1 : tiles)));
 // 16 positions a thread; 8 where a tile of 128 would be half empty (256 x 64 x 2048 bf16: 92 us with 16,
 // 56 with 8; 128 x 128 x 2048: 48 with 16, 63 with 8; 4 x 4096 x 2048: 57 and 69)
 #define DPK_SCAN_FWD(TT, VV)                                                                                           \
   do {                                                                                                                 \
-    if (T <= kChunk) hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 8>), grid, dim3(kThreads), 0, s, p);                  \
-    else hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 16>), grid, dim3(kThreads), 0, s, p);                             \
+    if (walk) hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 8, true>), grid, dim3(kThreads), 0, s, p);                  \
+    else if (T <= kChunk) hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 8, false>), grid, dim3(kThreads), 0, s, p);      \
+    else hipLaunchKernelGGL((scan_fwd_kernel<TT, VV, 16, false>), grid, dim3(kThreads), 0, s, p);                      \
   } while (0)
   if (dtype == DPK_BF16) {
     if (V == 2) DPK_SCAN_FWD(bf16_t, 2);
@@ -827,17 +886,22 @@ extern "C" int dpk_gated_scan_backward(const void* gates, int dtype, const void*
   const int V = vec_of(2, D, dtype, gates_stride_n, gates_stride_t, n, T, {gates, grad_out, grad_gates},
                        {kept, grad_last, grad_decay, grad_state});
   const int tiles = tiles_of(T, kBwdTile);
+  const bool walk = bwd_walks(n, T, D), parts = tiles > 1 && !walk && grad_decay;
   DPK_REQUIRE(dpk_grid_fits(n * dpk_cdiv(D, kCL * V) * tiles, kBwdThreads), DPK_E_SHAPE, "%s: n * T * D too large", fn);
-  const size_t need = chain_bytes(n, D, V, tiles) + (tiles > 1 && grad_decay ? static_cast<size_t>(tiles) * n * D * 4 : 0);
+  const size_t need = walk ? 0 : chain_bytes(n, D, V, tiles) + (parts ? static_cast<size_t>(tiles) * n * D * 4 : 0);
   DPK_REQUIRE(need == 0 || (ws && ws_bytes >= need), DPK_E_WORKSPACE, "%s: workspace too small (%zu < %zu)", fn, ws_bytes, need);
   DPK_REQUIRE(dpk_aligned(ws, 16), DPK_E_ALIGN, "%s: workspace not 16-byte aligned", fn);
   hipStream_t s = static_cast<hipStream_t>(stream);
   ScanBwdArgs p = {gates, decay, kept, lengths, grad_out, grad_last, grad_gates, grad_state, grad_decay, n, T, D,
                    gates_stride_n, gates_stride_t, decay_dtype == DPK_BF16, reverse, {}};
-  char* behind = chain_of(&p.ch, n, D, V, tiles, ws, s);
-  if (tiles > 1 && grad_decay) p.dlam = reinterpret_cast<float*>(behind);
-  const dim3 grid(static_cast<unsigned>(p.ch.rows * tiles));
-#define DPK_SCAN_BWD(TT, VV) hipLaunchKernelGGL((scan_bwd_kernel<TT, VV>), grid, dim3(kBwdThreads), 0, s, p)
+  char* behind = chain_of(&p.ch, n, D, V, tiles, walk, ws, s);
+  if (parts) p.dlam = reinterpret_cast<float*>(behind);
+  const dim3 grid(static_cast<unsigned>(p.ch.rows * (walk ? 1 : tiles)));
+#define DPK_SCAN_BWD(TT, VV)                                                                                \
+  do {                                                                                                      \
+    if (walk) hipLaunchKernelGGL((scan_bwd_kernel<TT, VV, true>), grid, dim3(kBwdThreads), 0, s, p);        \
+    else hipLaunchKernelGGL((scan_bwd_kernel<TT, VV, false>), grid, dim3(kBwdThreads), 0, s, p);            \
+  } while (0)
   if (dtype == DPK_BF16) {
     if (V == 2) DPK_SCAN_BWD(bf16_t, 2);
     else DPK_SCAN_BWD(bf16_t, 1);
@@ -846,7 +910,7 @@ extern "C" int dpk_gated_scan_backward(const void* gates, int dtype, const void*
     else DPK_SCAN_BWD(float, 1);
   }
 #undef DPK_SCAN_BWD
-  if (tiles > 1 && grad_decay)
+  if (parts)
     hipLaunchKernelGGL(scan_dlam_kernel, dim3(static_cast<unsigned>(dpk_cdiv(n * D, DPK_WAVE))),
                        dim3(DPK_WAVE * (tiles <= 32 ? 4 : 16)), 0, s, p.dlam, tiles, n * D, grad_decay);
   DPK_LAUNCH_CHECK(fn);

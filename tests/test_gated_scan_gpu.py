@@ -70,6 +70,28 @@ def test_gates_and_decays_over_their_whole_range(dtype):
     check(*make(3, 300, 48, dtype, with_state=True, wide=True))
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,T,D", [(3, 130, 66), (2, 192, 5), (4, 193, 64), (3, 256, 6), (2, 257, 64)])
+def test_lengths_around_the_longest_that_one_block_takes(n, T, D, dtype, reverse):
+    check(*make(n, T, D, dtype, ragged=True, with_state=True), reverse=reverse)
+
+
+# 512 blocks fill the GPU backward: every row by one block, whatever its length; 400 do not
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("n,T,D,dtype", [
+    (512, 300, 4, torch.float32), (500, 260, 3, torch.bfloat16), (64, 330, 512, torch.bfloat16), (400, 300, 4, torch.float32),
+    (171, 65, 130, torch.float32),
+])
+def test_rows_that_fill_the_gpu(n, T, D, dtype, ragged):
+    from opacus_amd import _lib
+
+    fills = n * -(-D // 64) >= 436
+    # (forward, 256 positions are the most that need no workspace)
+    assert (_lib.lib().dpk_gated_scan_workspace_bytes(n, min(T, 256), D) == 0) == (fills or T <= 192)
+    check(*make(n, T, D, dtype, ragged=ragged, with_state=ragged), reverse=ragged)
+
+
 def test_many_rows_leave_the_time_axis_whole():
     check(*make(40, 140, 1024, torch.bfloat16))
 
