@@ -996,6 +996,8 @@ def gated_scan_backward(
     ``gated_scan(..., keep_states=True)`` returned for the same gates, decay, lengths and direction;
     ``grad_last`` (float32) is the gradient of the last state."""
     dev, (n, T, D), decay, lengths, code, decay_code = _scan_args(gates, decay, lengths, 3)
+    if kept is None:
+        raise ValueError("kept must be what gated_scan(..., keep_states=True) returned")
     _need_gpu(gates, kept, grad_out)
     if grad_out.shape != (n, T, D):
         raise ValueError(f"grad_out must be {(n, T, D)}, got {tuple(grad_out.shape)}")

@@ -262,6 +262,8 @@ def test_refusals_on_the_gpu():
         kernels.gated_scan(gates, decay.cpu())
     with pytest.raises(ValueError, match="kept"):
         kernels.gated_scan_backward(gates, decay, kept[:, :0], dy)
+    with pytest.raises(ValueError, match="keep_states"):
+        kernels.gated_scan_backward(gates, decay, kernels.gated_scan(gates, decay)[2], dy)
     with pytest.raises(ValueError, match="grad_out"):
         kernels.gated_scan_backward(gates, decay, kept, dy[:, :3])
     with pytest.raises(ValueError, match="grad_last"):
