@@ -378,8 +378,12 @@ int dpk_layer_norm_gs(const void* x, const void* b, int in_dtype, void* gs_w, vo
  * state before every DPK_SCAN_CHUNK-th position in the order of the scan.
  * n == 0 or D == 0 launches nothing; T == 0 writes last only. Tensors need their element size's
  * alignment; wider alignment (and D, strides in multiples of 4 or 2) takes wider loads.
+ * 3 * D and, where T > 1, gates_stride_t are at most DPK_SCAN_MAX_STRIDE (offsets inside a tile of positions
+ * are 32 bits wide); more is DPK_E_SHAPE, and a caller copies such gates into dense ones. Nothing
+ * limits gates_stride_n.
  * ws: dpk_gated_scan_workspace_bytes bytes (one query for both directions), 16-byte aligned. */
 #define DPK_SCAN_CHUNK 64
+#define DPK_SCAN_MAX_STRIDE 4194303
 size_t dpk_gated_scan_workspace_bytes(int64_t n, int64_t T, int64_t D);
 int dpk_gated_scan(const void* gates, int dtype, const void* decay, int decay_dtype, const float* state,
                    const int64_t* lengths, void* out, float* last, float* kept, int64_t n, int64_t T, int64_t D,

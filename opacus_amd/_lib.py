@@ -24,6 +24,7 @@ DPK_ROUTE_AUTO, DPK_ROUTE_GRAM, DPK_ROUTE_DIRECT = 0, 1, 2
 DPK_STATIC_SCRATCH_BYTES = 8 << 20
 DPK_GHOST_MULTI_MAX = 256
 DPK_SCAN_CHUNK = 64
+DPK_SCAN_MAX_STRIDE = 4194303
 DPK_ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 

@@ -46,7 +46,8 @@ constexpr int kFwdTile = 128;            // forward: 16 positions per thread, or
 constexpr int kWalkTile = 64;
 static_assert(kBwdTile == kChunk && kFwdTile % kChunk == 0, "tiles start at kept states");
 // Byte offsets inside a tile are 32 bits wide.
-constexpr int64_t kMaxStride = (1LL << 31) / (kFwdTile * 4) - 1;
+constexpr int64_t kMaxStride = DPK_SCAN_MAX_STRIDE;
+static_assert(kMaxStride == (1LL << 31) / (kFwdTile * 4) - 1, "the largest offset inside a tile of fp32 fits 31 bits");
 
 // softplus(v) = max(v, 0) + log1p(exp(-|v|)), with log1p(e) = log(1 + e) * e / ((1 + e) - 1): the
 // quotient corrects what the rounding of 1 + e did, so the result keeps its relative accuracy as

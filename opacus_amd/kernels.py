@@ -907,8 +907,13 @@ def _at(t: Optional[torch.Tensor]):
 
 
 def _gates_layout(gates: torch.Tensor, D: int) -> Tuple[torch.Tensor, int, int]:
-    """``gates`` with unit stride along its features, and its sample and position strides."""
-    if gates.numel() and (gates.stride(-1) != 1 or min(gates.stride()) < 0):
+    """``gates`` with unit stride along its features, and its sample and position strides. Positions that
+    lie further apart than the kernels' offsets inside a tile reach are brought together by a copy."""
+    if gates.numel() and (
+        gates.stride(-1) != 1
+        or min(gates.stride()) < 0
+        or (gates.shape[1] > 1 and gates.stride(1) > _lib.DPK_SCAN_MAX_STRIDE)
+    ):
         gates = gates.contiguous()
     n, T = gates.shape[0], gates.shape[1]
     return gates, (gates.stride(0) if n > 1 else T * 3 * D), (gates.stride(1) if T > 1 else 3 * D)
@@ -962,7 +967,9 @@ def gated_scan(
     (float32 ``[n, D]``) comes before the first position. ``lengths`` (int64 ``[n]``) marks
     positions from ``lengths[b]`` on as padding, which is never read: the state passes over it and
     the output is zero there. ``reverse`` scans from the last position to the first. ``gates``
-    may be a slice of a larger tensor (any strides but along the features)."""
+    may be a slice of a larger tensor: it is read in place whatever its strides, but copied where its
+    features are not dense or its positions lie more than ``_lib.DPK_SCAN_MAX_STRIDE`` elements
+    apart (a ``[T, n, 3 D]`` storage of very many samples). ``3 D`` may not exceed that number either."""
     dev, (n, T, D), decay, lengths, code, decay_code = _scan_args(gates, decay, lengths, 3)
     state = _scan_state("state", state, (n, D), dev)
     out = gates.new_empty(n, T, D)

@@ -109,3 +109,24 @@ def test_wrappers_take_gpu_tensors_only():
         kernels.gated_scan_backward(gates, decay, torch.zeros(1, 1, 2), torch.zeros(1, 2, 2))
     with pytest.raises(RuntimeError, match="GPU only"):
         kernels.gated_scan_step(gates[:, 0], decay, torch.zeros(1, 2))
+
+
+def test_positions_too_far_apart_for_the_kernels_are_copied():
+    """A [T, n, 3 D] storage seen as [n, T, 3 D] has n * 3 D elements between positions, which may be more than
+    the kernels' 32-bit offsets inside a tile reach."""
+    from opacus_amd import _lib, kernels
+
+    most, D = _lib.DPK_SCAN_MAX_STRIDE, 4
+    for stride, kept in ((most, True), (most + 1, False), (2 * most, False)):
+        gates = torch.empty_strided((2, 3, 3 * D), (3 * D, stride, 1), device="meta")
+        view, sn, st = kernels._gates_layout(gates, D)
+        assert (view is gates) == kept and (sn, st) == ((3 * D, stride) if kept else (9 * D, 3 * D))
+    one = torch.empty_strided((2, 1, 3 * D), (3 * D, 2 * most, 1), device="meta")  # no second position
+    assert kernels._gates_layout(one, D)[0] is one
+    # the C entry points say so
+    L, at, SHAPE, WS = _lib.lib(), 4096, -1, -5
+    for st, code in ((most, WS), (most + 1, SHAPE)):
+        assert L.dpk_gated_scan(at, 0, at, 0, None, None, at, at, None, 1, 4096, D, 12, st, 0, None, 0, None) == code
+        assert L.dpk_gated_scan_backward(
+            at, 0, at, 0, at, None, at, None, at, None, None, 1, 4096, D, 12, st, 0, None, 0, None
+        ) == code
