@@ -26,7 +26,7 @@ from torch.nn.utils.rnn import PackedSequence
 from .. import kernels
 from .dp_rnn import RNNLinear, apply_permutation
 from .norm_act import HeadNormAct
-from .param_rows import first_derivative_only, parameter_rows
+from .param_rows import first_derivative_only, forget_rows, parameter_rows
 
 
 class _GatedScanFn(torch.autograd.Function):
@@ -83,7 +83,11 @@ class GatedScan(nn.Module):
         if torch.is_grad_enabled() and self.decay.requires_grad:
             rows = parameter_rows(self, (self.decay,), gates.shape[0])
         state = None if state is None else state.float()
-        out, last = _GatedScanFn.apply(wide, rows, state, kernels.widen(self.decay.detach()), lengths, self.reverse)
+        try:
+            out, last = _GatedScanFn.apply(wide, rows, state, kernels.widen(self.decay.detach()), lengths, self.reverse)
+        except BaseException:
+            forget_rows(self)
+            raise
         return (out if out.dtype == gates.dtype else out.to(gates.dtype)), last
 
     @torch.no_grad()

@@ -15,7 +15,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .. import _lib, kernels
-from .param_rows import first_derivative_only, parameter_rows, rows_dim
+from .param_rows import first_derivative_only, forget_rows, parameter_rows, rows_dim
 
 
 class _NormActFn(torch.autograd.Function):
@@ -91,7 +91,11 @@ class _NormAct(nn.Module):
         if self.affine and torch.is_grad_enabled() and (self.weight.requires_grad or self.bias.requires_grad):
             rows = parameter_rows(self, (self.weight, self.bias), x.shape[0])
         weight, bias = (None, None) if not self.affine else (kernels.widen(self.weight.detach()), kernels.widen(self.bias.detach()))
-        y = _NormActFn.apply(wide, rows, weight, bias, self.num_groups, self.eps, self.activation, self.per_position)
+        try:
+            y = _NormActFn.apply(wide, rows, weight, bias, self.num_groups, self.eps, self.activation, self.per_position)
+        except BaseException:
+            forget_rows(self)
+            raise
         return y if y.dtype == x.dtype else y.to(x.dtype)
 
 

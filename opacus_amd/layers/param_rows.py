@@ -27,6 +27,12 @@ def parameter_rows(module: nn.Module, params: Sequence[nn.Parameter], n: int) ->
     return rows
 
 
+def forget_rows(module: nn.Module) -> None:
+    """For a forward pass that raises after :func:`parameter_rows`: no hook picks its rows up, and a tensor
+    that is left on the module keeps it from being copied."""
+    module.__dict__.pop("_dpk_param_rows", None)
+
+
 def rows_dim(module: nn.Module) -> int:
     """The dimension of ``module``'s input that the samples lie along: 0, or 1 where the grad-sample hooks
     of a model with ``batch_first=False`` are installed on a layer that follows the model's layout

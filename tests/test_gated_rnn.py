@@ -1,5 +1,7 @@
 """DPGatedRNN, GroupNormAct and HeadNormAct on the CPU: construction, names, refusals, hook wiring."""
 
+import copy
+
 import pytest
 import torch
 import torch.nn as nn
@@ -78,3 +80,16 @@ def test_rows_are_kept_for_hooked_modules_only():
     assert rows.shape == (0, 2, 4)
     rows.sum().backward()
     assert (norm.weight.grad == 0).all()
+
+
+@pytest.mark.parametrize("make", [lambda: GatedScan(4), lambda: HeadNormAct(2, 12), lambda: GroupNormAct(3, 12)])
+@pytest.mark.parametrize("cls", [GradSampleModule, GradSampleModuleFastGradientClipping])
+def test_a_refused_call_leaves_nothing_on_the_module(cls, make):
+    """A wrapped model whose forward pass raised (here: CPU tensors) can still be copied and used."""
+    module = make()
+    wrapped = cls(module)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        wrapped(torch.zeros(2, 12, 12))
+    assert "_dpk_param_rows" not in module.__dict__ and not getattr(module, "activations", [])
+    other = copy.deepcopy(module)
+    assert all(torch.equal(p, q) for p, q in zip(module.parameters(), other.parameters()))
