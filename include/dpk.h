@@ -393,7 +393,9 @@ int dpk_gated_scan(const void* gates, int dtype, const void* decay, int decay_dt
 /* Gradients of the above from grad_out: [n,T,D] of `dtype` (dense) and grad_last: float[n,D] or
  * NULL. grad_gates: [n,T,3D] of `dtype` (dense, zero at padding). grad_decay (nullable): float[n,D],
  * the PER-SAMPLE gradient of decay, which the same pass yields. grad_state (nullable): float[n,D].
- * gates, decay, lengths, reverse as given to dpk_gated_scan, kept as it left it. */
+ * gates, decay, lengths, reverse as given to dpk_gated_scan, kept as it left it. The same call gives the
+ * same bits every time; a sample's gradients may differ in their last bits from one n to another (sums are
+ * formed in another order where rows fill the GPU). */
 int dpk_gated_scan_backward(const void* gates, int dtype, const void* decay, int decay_dtype, const float* kept,
                             const int64_t* lengths, const void* grad_out, const float* grad_last, void* grad_gates,
                             float* grad_decay, float* grad_state, int64_t n, int64_t T, int64_t D,

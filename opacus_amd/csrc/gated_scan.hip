@@ -8,8 +8,10 @@
 // tile of positions for 32 * V channels of a sample: every thread runs K positions of its channels in
 // registers, the block's time groups exchange their (A, B) through lanes and LDS, and the tiles of a
 // row pass the state on in one launch (see "the chain" below), or one block walks through all of them where
-// that is faster (bwd_walks), so every input is read once and every output written once. What is folded, and in which order, depends on sizes alone: the same bits on
-// every run.
+// that is faster (bwd_walks), so every input is read once and every output written once. What is folded, and in which
+// order, depends on sizes and alignment alone: the same bits on every run. n is among the sizes backward (bwd_walks), so a
+// sample's gradients are not the same bits in every batch: a walking thread adds up the decay's gradient over all of its
+// positions, the chain tile by tile.
 //
 // Backward: g_t = dy_t + a_{t+1} g_{t+1} runs the same maps the other way (same A, other B), and
 //   q = 1 - a,  m = sqrt(q (1 + a)),  kappa = -L / m,  s = sigma(i)

@@ -1001,7 +1001,8 @@ def gated_scan_backward(
     grad_state [n, D])``, the last two in float32. ``grad_decay`` is the per-sample gradient of
     ``decay``: the pass that forms the gate gradients has it on the way. ``kept`` is what
     ``gated_scan(..., keep_states=True)`` returned for the same gates, decay, lengths and direction;
-    ``grad_last`` (float32) is the gradient of the last state."""
+    ``grad_last`` (float32) is the gradient of the last state. The same call gives the same bits every
+    time, but a sample's gradients may differ in their last bits between batch sizes."""
     dev, (n, T, D), decay, lengths, code, decay_code = _scan_args(gates, decay, lengths, 3)
     if kept is None:
         raise ValueError("kept must be what gated_scan(..., keep_states=True) returned")

@@ -106,7 +106,8 @@ def scan_reference(gates, decay, state=None, lengths=None, reverse=False, grad_o
     ratio = torch.sigmoid(lam) / sp
     w, w_t = torch.where(mask, w, zero), torch.where(mask, w_t, zero)
     val["grad_decay"] = w.sum(1) * ratio
-    # the sum over positions: at most T roundings, in practice a few dozen in a row
+    # the sum over positions: at most T roundings (a few dozen in a row where a row is a chain of tiles; T / 8 and
+    # a few where one block walks it)
     tol["grad_decay"] = (w_t.sum(1) + H * (T + 30) * w.abs().sum(1)) * ratio
     val["grad_state"], tol["grad_state"] = R, Re + H * Rabs
     return val, tol

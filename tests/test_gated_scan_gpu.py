@@ -415,3 +415,35 @@ def test_positions_far_apart(beyond, dtype, reverse):
     view = storage.as_strided((2, 131, 192), (192, stride, 1))
     view.copy_(gates)
     check(view, decay, state, lengths, dy, dl, reverse)
+
+
+def test_a_sample_alone_and_in_a_batch_that_fills_the_gpu():
+    """Backward, 512 rows are walked by a block each, where one row of the same length is a chain of tiles. The states are
+    the same bits (forward depends on T alone); the gradients are sums in another order, most of all that of the decay,
+    which the walk adds up over all of a thread's positions and the chain tile by tile: each within its bound,
+    not the same bits."""
+    from opacus_amd import _lib, kernels
+
+    n, T, D, k = 512, 300, 4, 317
+    L = _lib.lib()  # (256 positions: the longest that one block takes forward, so only backward may need a workspace)
+    assert L.dpk_gated_scan_workspace_bytes(n, 256, D) == 0 and L.dpk_gated_scan_workspace_bytes(1, 256, D) > 0
+    gates, decay, state, lengths, dy, dl = make(n, T, D, torch.float32, ragged=True, with_state=True)
+    lengths[k] = T - 7
+    batch = (gates, decay, state, lengths, dy, dl)
+    one = (gates[k : k + 1], decay, state[k : k + 1], lengths[k : k + 1], dy[k : k + 1], dl[k : k + 1])
+    val, tol = scan_reference(one[0], decay, one[2], one[3], False, one[4], one[5])
+    runs = []
+    for (g, d, s, l, y, z), at in ((batch, k), (one, 0)):
+        out, last, kept = kernels.gated_scan(g, d, s, l, keep_states=True)
+        runs.append([t[at : at + 1] for t in (out, last, kept) + kernels.gated_scan_backward(g, d, kept, y, z, l)])
+    for p, q in zip(runs[0][:3], runs[1][:3]):
+        assert torch.equal(p, q)
+    for run in runs:
+        for name, got in zip(("grad_gates", "grad_decay", "grad_state"), run[3:]):
+            assert_within(got, val[name], tol[name], name)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_a_long_row_walked_by_one_block(reverse):
+    """47 tiles in turn: a thread adds up 375 positions of the decay's gradient in a row (the bound allows T)."""
+    check(*make(512, 3000, 2, torch.float32, ragged=True, with_state=True), reverse=reverse)
