@@ -227,3 +227,24 @@ def test_offsets_past_32_bits():
     assert (dw[1] - dw1[0]).abs().max() <= 2 * bar * S and (db[1] - db1[0]).abs().max() <= 2 * bar * S
     # outputs: at most a rounding apart (2**-8 of values below 16 and of gradients below 16)
     assert (y[1] - y1[0]).abs().max() <= 2.0**-4 and (dx[1] - dx1[0]).abs().max() <= 2.0**-4
+
+
+# 64 channels in 32 groups: one block holds a slab of up to 512 positions in bfloat16, 1024 in float32; beyond it the
+# statistics, their merge and the application are launches of their own
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("S,dtype", [
+    (512, torch.bfloat16), (513, torch.bfloat16), (1024, torch.float32), (1025, torch.float32),
+])
+def test_both_sides_of_the_longest_slab(S, dtype, act):
+    check(*make(2, S, 64, dtype), 32, act, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,S,C,groups", [(3, 16, 2048, 1), (2, 8, 2040, 1), (2, 3, 2046, 2), (3, 16, 1000, 1), (2, 64, 512, 2)])
+def test_wide_groups_within_one_block(n, S, C, groups, dtype, monkeypatch):
+    """One thread adds up a group's channels, so the longest path is the group's width, after 16 positions and up to 512
+    row groups."""
+    import _norm_act_reference
+
+    monkeypatch.setattr(_norm_act_reference, "P", C // groups + 16 + 512)
+    check(*make(n, S, C, dtype), groups, "silu", False)
