@@ -6,6 +6,7 @@ position (40 * 12 * 2**-24 = 2.9e-5), a second layer the same, the products of t
 terms) and the norms less than that: 1e-4 at every scale of tests/_compare.py."""
 
 import copy
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -475,3 +476,181 @@ def test_samples_along_the_second_dimension(T, reduction):
     assert_rel(ghost.get_norm_sample()[None], norms[None], REL, "norms")
     with pytest.raises(ValueError, match="batch_first=False"):
         wrapped._module.norm(torch.zeros(5, 24, device="cuda"))
+
+
+# ---- what an optimizer step leaves, with no noise in it -------------------------------------------
+def clipped_sum(want, C):
+    norms = torch.stack([g.flatten(1).norm(dim=1) for g in want.values()]).norm(dim=0)
+    coef = (C / (norms + 1e-6)).clamp(max=1.0)
+    return norms, {k: torch.einsum("n,n...->...", coef, g) for k, g in want.items()}
+
+
+@pytest.mark.parametrize("mode", ["hooks", "ghost"])
+def test_make_private_without_noise_applies_the_clipped_sum(mode):
+    """Poisson batches, the update against the formula's; then an empty batch, which changes nothing."""
+    from opacus_amd import PrivacyEngine
+
+    torch.manual_seed(14)
+    net = Net(1, False, 4)
+    ref = copy.deepcopy(net)
+    net = net.cuda()
+    ids, y = data(16, 9)
+    loader = torch.utils.data.DataLoader(torch.utils.data.TensorDataset(ids, y), batch_size=8)
+    settings = dict(
+        module=net, optimizer=torch.optim.SGD(net.parameters(), lr=0.05), data_loader=loader, noise_multiplier=0.0,
+        max_grad_norm=0.5, grad_sample_mode=mode,
+    )
+    if mode == "hooks":
+        model, opt, loader = PrivacyEngine().make_private(**settings)
+        crit = nn.CrossEntropyLoss()
+    else:
+        model, opt, crit, loader = PrivacyEngine().make_private(criterion=nn.CrossEntropyLoss(), **settings)
+    batches = [(bi, by) for bi, by in loader if len(bi)][:3] + [(ids[:0], y[:0])]
+    assert len(batches) > 1
+    for bi, by in batches:
+        before = {k: p.detach().clone() for k, p in net.named_parameters()}
+        opt.zero_grad()
+        crit(model(bi.cuda()), by.cuda()).backward()
+        if len(bi) == 0:
+            if mode == "hooks":
+                assert all(p.grad_sample.shape[0] == 0 for p in net.parameters())
+            else:
+                assert model.per_sample_gradient_norms.shape == (0,)
+            opt.step()
+            assert all(torch.equal(p, before[k]) for k, p in net.named_parameters())
+            continue
+        ref.load_state_dict({k: v.cpu() for k, v in before.items()})
+        norms, want = clipped_sum(per_sample_reference(ref, bi, by), 0.5)
+        assert (norms > 0.5).any()
+        opt.step()
+        for k, p in net.named_parameters():
+            assert_rel(p.grad.reshape(1, -1), want[k].reshape(1, -1) / 8, REL, k)
+            # the product and the difference, each rounded once
+            step = 0.05 * p.grad.double()
+            assert ((p.double() - (before[k].double() - step)).abs() <= 2**-23 * (before[k].double().abs() + step.abs())).all()
+
+
+@pytest.mark.parametrize("channels_last", [False, True])
+@pytest.mark.parametrize("single", [True, False])
+def test_group_norm_act_under_ghost_clipping(single, channels_last):
+    from opacus_amd import GradSampleModuleFastGradientClipping
+    from opacus_amd.layers import GroupNormAct
+    from opacus_amd.optimizers import DPOptimizerFastGradientClipping
+    from opacus_amd.utils.fast_gradient_clipping_utils import DPLossFastGradientClipping
+
+    torch.manual_seed(15)
+
+    class Block(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.conv, self.norm, self.fc = nn.Conv2d(3, 16, 3, padding=1), GroupNormAct(4, 16, activation="gelu"), nn.Linear(16, 5)
+
+        def forward(self, x):
+            return self.fc(self.norm(self.conv(x)).mean((2, 3)))
+
+        def reference(self, x, _length):
+            return self.fc(ref_norm(self.norm, F.conv2d(x, self.conv.weight, self.conv.bias, padding=1)).mean((2, 3)))
+
+    net = Block()
+    with torch.no_grad():
+        net.norm.weight.add_(0.2 * torch.randn(16))
+        net.norm.bias.add_(0.2 * torch.randn(16))
+    x, y = torch.randn(5, 3, 7, 9), torch.randint(0, 5, (5,))
+    want = per_sample_reference(net, x.double(), y)
+    C = float(torch.stack([g.flatten(1).norm(dim=1) for g in want.values()]).norm(dim=0).median())
+    norms, total = clipped_sum(want, C)
+    model = GradSampleModuleFastGradientClipping(net.cuda(), loss_reduction="mean", max_grad_norm=C, single_backward=single)
+    opt = DPOptimizerFastGradientClipping(
+        torch.optim.SGD(net.parameters(), lr=0.1), noise_multiplier=0.0, max_grad_norm=C, expected_batch_size=5
+    )
+    crit = DPLossFastGradientClipping(model, opt, nn.CrossEntropyLoss(), loss_reduction="mean")
+    xin = x.cuda().contiguous(memory_format=torch.channels_last) if channels_last else x.cuda()
+    for _ in range(2):
+        opt.zero_grad()
+        crit(model(xin), y.cuda()).backward()
+        assert_rel(model.per_sample_gradient_norms, norms, REL, "norms")
+        for name, p in net.named_parameters():
+            assert_rel(p.grad.reshape(1, -1), total[name].reshape(1, -1), REL, name)
+
+
+# ---- initial states, dropout ----------------------------------------------------------------------
+def rnn_rows(ref, seqs, state, middle=None):
+    """Per sample: outputs, last states, gradients of the state and of every parameter, for the loss
+    ``sum out^2 + sum h * (1, 2, ..)``. ``middle[k]``: what dropout multiplies sample k's second layer's input by."""
+    res = []
+    weight = torch.arange(1.0, 1 + len(ref.cells), dtype=torch.float64)[:, None, None]
+    for k, s in enumerate(seqs):
+        ref.zero_grad(set_to_none=True)
+        init = state[:, k : k + 1].detach().clone().double().requires_grad_(True)
+        if middle is None:
+            o, h = ref_rnn(ref, s[None].double(), init)
+        else:
+            half = ref.num_directions
+            first, last = (SimpleNamespace(num_layers=1, num_directions=half, cells=c) for c in (ref.cells[:half], ref.cells[half:]))
+            o, h0 = ref_rnn(first, s[None].double(), init[:half])
+            o, h1 = ref_rnn(last, o * middle[k : k + 1], init[half:])
+            h = torch.cat([h0, h1])
+        (o.pow(2).sum() + (h * weight).sum()).backward()
+        res.append((o[0].detach(), h.detach(), init.grad, {n: p.grad.clone() for n, p in ref.named_parameters()}))
+    return res
+
+
+def check_rnn(rnn, out_rows, h, state, res):
+    for k, (o, hk, gk, _) in enumerate(res):
+        assert_rel(out_rows[k], o, REL, f"output {k}")
+        assert_rel(h[:, k : k + 1], hk, REL, f"last state {k}")
+        assert_rel(state.grad[:, k : k + 1], gk, REL, f"gradient of state {k}")
+    for name, p in rnn.named_parameters():
+        assert_rel(p.grad_sample, torch.stack([r[3][name] for r in res]), REL, name)
+
+
+def rnn_loss(data_, h):
+    return data_.pow(2).sum() + (h * torch.arange(1.0, 1 + len(h), device=h.device)[:, None, None]).sum()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("batch_first", [False, True])
+def test_initial_states_of_every_layer_and_direction(batch_first, packed):
+    from opacus_amd import GradSampleModule
+
+    torch.manual_seed(16)
+    rnn = DPGatedRNN_(6, 24, 2, True, 4, batch_first)
+    lens = [4, 9, 1, 8] if packed else [7] * 4  # (packed order: samples 1, 3, 0, 2)
+    seqs, start = [torch.randn(k, 6) for k in lens], torch.randn(4, 4, 24)
+    res = rnn_rows(copy.deepcopy(rnn).double(), seqs, start)
+    model = GradSampleModule(rnn.cuda(), batch_first=batch_first, loss_reduction="sum")
+    state = start.cuda().requires_grad_(True)
+    if packed:
+        out, h = model(nn.utils.rnn.pack_sequence([s.cuda() for s in seqs], enforce_sorted=False), state)
+        rnn_loss(out.data, h).backward()
+        padded = nn.utils.rnn.pad_packed_sequence(out, batch_first=True)[0]
+        rows = [padded[k, :n] for k, n in enumerate(lens)]
+    else:
+        x = torch.stack(seqs, 0 if batch_first else 1).cuda()
+        out, h = model(x, state)
+        rnn_loss(out, h).backward()
+        rows = out if batch_first else out.transpose(0, 1)
+    check_rnn(rnn, rows, h, state, res)
+
+
+def test_dropout_acts_between_the_layers_only():
+    from opacus_amd import GradSampleModule
+    from opacus_amd.layers import DPGatedRNN
+
+    torch.manual_seed(17)
+    rnn = DPGatedRNN(6, 24, 2, batch_first=True, dropout=0.5, num_heads=4)
+    seqs, start = [torch.randn(7, 6) for _ in range(3)], torch.randn(2, 3, 24)
+    ref = copy.deepcopy(rnn).double()
+    model = GradSampleModule(rnn.cuda(), loss_reduction="sum")
+    kept = []
+    rnn.dropout_layer.register_forward_hook(lambda _m, _i, o: kept.append((o != 0).double().cpu() * 2))
+    state = start.cuda().requires_grad_(True)
+    out, h = model(torch.stack(seqs).cuda(), state)
+    rnn_loss(out, h).backward()
+    assert len(kept) == 1 and 0.2 < float(kept[0].mean()) / 2 < 0.8
+    check_rnn(rnn, out, h, state, rnn_rows(ref, seqs, start, kept[0]))
+    model.eval()
+    with torch.no_grad():
+        out, _ = model(torch.stack(seqs).cuda(), state)
+    for k, (o, *_rest) in enumerate(rnn_rows(ref, seqs, start)):
+        assert_rel(out[k], o, REL, f"output {k} in evaluation")
