@@ -381,7 +381,8 @@ int dpk_layer_norm_gs(const void* x, const void* b, int in_dtype, void* gs_w, vo
  * 3 * D and, where T > 1, gates_stride_t are at most DPK_SCAN_MAX_STRIDE (offsets inside a tile of positions
  * are 32 bits wide); more is DPK_E_SHAPE, and a caller copies such gates into dense ones. Nothing
  * limits gates_stride_n.
- * ws: dpk_gated_scan_workspace_bytes bytes (one query for both directions), 16-byte aligned. */
+ * ws: dpk_gated_scan_workspace_bytes bytes, 16-byte aligned. One query for both directions: a forward
+ * pass alone uses less than half of it. */
 #define DPK_SCAN_CHUNK 64
 #define DPK_SCAN_MAX_STRIDE 4194303
 size_t dpk_gated_scan_workspace_bytes(int64_t n, int64_t T, int64_t D);

@@ -22,16 +22,20 @@
 // again from the fp32 state the forward pass kept at every 64th position, so no rounded output
 // enters a gradient.
 //
-// Bounds, at 16 x 1024 x 2048: forward bf16 54 us for 272 MB (5.0 TB/s; a large copy reaches 4.9 to 5.3), fp32 110 us
-// for 541 MB (4.9 TB/s): memory. Backward fp32 187 us for 948 MB (5.1 TB/s): memory. Backward bf16 109 us for 478 MB
-// (4.4 TB/s): half the cycles issue arithmetic (62 vector instructions an element, 6 of them transcendental),
-// and the two waves a SIMD that their registers leave cover the loads for the rest. There a block walks; in the
-// chain it is 119 us, about 10 of them its clearing and the sum of the decay gradients. Tried for the walk and
-// slower: the next tile's inputs sent ahead into registers (116 us, fp32 242), three waves (129 us). For the chain:
+// Bounds, at 16 x 1024 x 2048, kernels alone, inputs in no cache: forward bf16 59 us for 272 MB (4.6 TB/s; a large copy
+// reaches 4.9 to 5.4), fp32 110 us for 541 MB (4.9 TB/s): memory. Backward fp32 187 us for 948 MB (5.1 TB/s): memory.
+// Backward bf16 106 us for 478 MB (4.5 TB/s) in a loop of such calls, 101 us among other kernels: half the cycles issue
+// arithmetic (55 vector instructions an element, 5 of them transcendental), and the two waves a SIMD that their
+// registers leave cover the loads for the rest. There a block walks: 109 us a call in a loop, in the chain 119, about 10
+// of them its clearing and the sum of the decay gradients. Tried for the walk and slower (us a call in that loop): the
+// next tile's inputs sent ahead into registers (116 us, fp32 242), three waves (129 us). For the chain:
 // 4 positions a thread in blocks of 512 (four waves a SIMD, 130 us), two waves with nothing spilled (134 us),
 // four with spills (211 us against 126 then), two rows a block with the second one's inputs sent ahead into
-// LDS (140 us against 126 then). One 16384-token row of 2048 channels: 68 us for 268 MB; a summary launch in front
-// instead of the chain took 127 us.
+// LDS (140 us against 126 then). One 16384-token row of 2048 channels: 66 us for 268 MB (4.1 TB/s), with the clearing
+// and the launches 80 us a call (70 with the same inputs call after call; a summary launch in front instead of the
+// chain took 127 us then).
+// Spills: the chain forward in bf16 4 registers (of the 128 that four waves a SIMD have), the chain backward 7 in bf16
+// and 6 in fp32 (of the 168 that three have).
 #include <initializer_list>
 
 #include "vec_io.h"
@@ -102,7 +106,8 @@ __device__ __forceinline__ float inv_scale(float q2) { return __builtin_amdgcn_r
 // never depends on timing, so the bits repeat; the serial part of a row is one hop per run.
 // A word is 64 bits, stored and read whole at agent scope (the XCDs' L2s are not coherent), with
 // the pattern kEmpty in its low half until it is written; a NaN is published as the usual quiet one.
-// (One row of 128 tiles of 2048 channels: 68 us with runs of 16, 70 with 8, 32 or 64; two rows backward: 123, 125, 124, 132.)
+// (One row of 128 tiles of 2048 channels, same inputs: 68 us with runs of 16, 70 with 8, 32 or 64; two rows backward:
+// 123, 125, 124, 132.)
 constexpr int kRun = 16;
 constexpr uint32_t kEmpty = 0xffffffffu;
 

@@ -15,10 +15,11 @@
 // holds, and put together from (count, mean, M2) triples, so that a large mean costs no digits.
 // All arithmetic is fp32; every reduction runs in a fixed order.
 //
-// Training passes (forward and backward): 256 x 1024 x 64 fp32, 32 groups: 67 us for 336 MB (5.0 TB/s), memory; per
-// position 16 x 1024 x 2048 bf16, 16 heads: 72 us for 335 MB (4.6 TB/s), memory and, backward, arithmetic (three
-// quarters of the issue slots); 3 x 40000 x 128 bf16, 32 groups, gelu: 80 us for 215 MB in six launches, half of the
-// issue slots arithmetic (gelu takes about 23 instructions a value in each of three passes), 10 us merges.
+// Training passes (forward and backward), inputs that change from pass to pass: 256 x 1024 x 64 fp32, 32 groups: 81 us
+// for 336 MB (kernels 24 and 44 us, 4.9 TB/s), memory; per position 16 x 1024 x 2048 bf16, 16 heads: 76 us for 335 MB
+// (kernels 28, 46 and 5 us), memory and, backward, arithmetic (three quarters of the issue slots); 3 x 40000 x 128 bf16,
+// 32 groups, gelu: 81 us in six launches that move eight streams of 31 MB (x; x, y; x, dy; x, dy, dx: 50 us at 4.9 TB/s),
+// half of the issue slots arithmetic (gelu takes about 23 instructions a value in each of three passes), 10 us merges.
 #include <type_traits>
 
 #include "vec_io.h"
@@ -34,7 +35,8 @@ constexpr int kRelu = DPK_ACT_RELU, kSilu = DPK_ACT_SILU, kGelu = DPK_ACT_GELU;
 
 // Phi(z) = (1 + erf(z / sqrt 2)) / 2 and E = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun:
 // erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2) with t = 1 / (1 + p x), off by at most 1.5e-7. Its
-// exponential is the one act' needs, and for z < 0 no 1 - erf cancels.
+// exponential is the one act' needs, and for z < 0 no 1 - erf cancels. Against the exact gelu that is 7e-7 of the value
+// for |z| < 1 (the erf form in fp32: 2e-7) and 2e-7 absolute below -1 (5e-8), so 5e-5 of the value at -3.
 __device__ __forceinline__ float normal_cdf(float z, float& E) {
   const float x = fabsf(z) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
@@ -470,12 +472,16 @@ __global__ __launch_bounds__(kThreads) void sample_dx_kernel(NormArgs p) {
 // fp32: 23 us forward and 44 us backward, against 73 and 74 us with partial sums, their merge and a second
 // reading (three launches each); 33 x 49 x 210: 7 us against 21. Slabs of 64 bytes, two blocks a CU instead of one:
 // 29 and 59 us.
+// What a thread holds ends the route: 64 values, so 1024 positions of 64 channels in 32 groups in fp32 and 512 in bf16.
+// A call forward and backward, on its two sides: 256 x 1024 x 64 fp32 24 and 49 us, 1088 positions 49 and 87; 256 x 512 x
+// 64 bf16 15 and 19 us, 1024 positions 34 and 61.
 constexpr int kSlabThreads = 512;
-constexpr int kSlabWidth = 2048;  // channels at most: 56 KB of LDS
+constexpr int kSlabWidth = 2048;  // channels at most: 40 KB of LDS with 16 KB for the row groups of 8-element vectors
 
 // s[i] (i < groups of the slab) = sum over the slab's channels i * Cg ... of w * v, v[V] being this
 // thread's value for its columns: first over the row groups, then over the channels. `chan` keeps the
-// channels' unweighted sums. lds: [step][W].
+// channels' unweighted sums. lds: [step][W]. One thread adds up a group's channels, which is nothing for a few and
+// most of the time for very wide groups: 64 x 16 x 2048 fp32 takes 26 us forward in 32 groups and 169 us in one.
 template <int V>
 __device__ __forceinline__ void slab_sums(const float (&v)[V], bool on, int rg, int lane, int step, int W, int Cg, float* lds,
                                           float* chan, float* s, const float* w) {
@@ -841,6 +847,10 @@ __global__ __launch_bounds__(kThreads, NI * V <= 8 ? 3 : 1) void position_rows_k
 }
 
 // ---- statistics per position, groups that no wave holds: one wave per (row, group) ---------------
+//
+// The simplest form: single elements, x read three times and more (from a cache after the first). 8 x 1024 x 4096 in one
+// group, forward and backward: bf16 83 and 235 us (floor 27 and 41), fp32 116 and 282 (55 and 82); 16 x 1024 x 2048 fp32
+// in one group 110 and 253, where the bf16 row, which a wave holds, takes 29 and 62.
 
 template <typename T, bool BACKWARD>
 __global__ __launch_bounds__(kThreads) void position_kernel(NormArgs p) {
@@ -915,7 +925,8 @@ __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(NormArgs p) {
 
 // The cut of [S, C] into blocks: a block covers up to 256 vectors of a row and as many rows at once as
 // its threads allow; S is cut into enough chunks to fill the GPU. `sums`: the chunks leave partial sums
-// of 8 bytes a channel, and none has less than 64 rows, or 8 for a thread.
+// of 8 bytes a channel, and there are no more of them than it takes to give each 64 rows, or 8 for a thread (rounded up
+// and then evened out: of 65 rows, two chunks of 33).
 void plan(NormArgs* p, int V, bool sums) {
   const int vecs = p->C / V;
   p->cl = vecs < kThreads ? vecs : kThreads;
@@ -977,8 +988,9 @@ bool plan_rows(NormArgs* p, int dtype, bool backward, int* V, int* NI) {
   for (p->wide = 1; p->wide < p->G && p->wide * p->lg < DPK_WAVE;) p->wide *= 2;
   p->cblocks = static_cast<int>(dpk_cdiv(p->G, p->wide));
   const int64_t rows = backward ? p->S : p->n * p->S, samples = backward ? p->n : 1;
-  // enough blocks to fill the GPU; backward, no chunk below 64 rows, nor 32 for every one that lies side by
-  // side in a wave (the partial sums of a chunk cost 8 bytes a channel and a reduction over the block)
+  // enough blocks to fill the GPU; backward, no more chunks than chunks of 64 rows, or of 32 for every one that lies side
+  // by side in a wave, would be, evened out (the partial sums of a chunk cost 8 bytes a channel and a reduction over the
+  // block)
   int64_t J = dpk_cdiv(backward ? 768 : kWantBlocks, samples * p->cblocks);
   const int64_t side = DPK_WAVE / (p->lg * p->wide);
   const int64_t most = dpk_cdiv(rows, !backward ? 4 * side : side > 2 ? 32 * side : 64);

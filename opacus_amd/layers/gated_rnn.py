@@ -129,7 +129,9 @@ class DPGatedRNN(nn.Module):
 
     ``lengths`` (int64 ``[B]`` on the inputs' device) marks a padded tensor's positions from
     ``lengths[b]`` on as padding, without the reordering of a ``PackedSequence``: the recurrence
-    passes over them (its outputs there are zero, and ``silu(bias)`` behind the norm).
+    passes over them (its outputs there are zero, and ``silu(bias)`` behind the norm). A ``PackedSequence``
+    is spread out and gathered again with masks, for which the host waits and which cannot be captured into a
+    graph; ``lengths`` have neither drawback.
     ``num_heads`` normalises every head of each output and applies SiLU."""
 
     def __init__(
